@@ -399,6 +399,105 @@ int sinter_argmax_ws_create(uint32_t blocks, int32_t *pass_cell, int32_t *histor
                             uint32_t history_cap, sinter_argmax_ws **out_dev);
 void sinter_argmax_ws_destroy(sinter_argmax_ws *dev);
 
+/* ------------------------------------------------------------------ 4-bit paged KV cache */
+/* Operators over a KV cache of 4-bit codes that a batch of sequences shares in
+ * pages: the per-token work around SINTER_OP_ATTN_DECODE's (q/k norm and rope,
+ * KV append, attention, gate; k0/ops/attn.cuh:119-488) for many sequences and
+ * any number of new tokens each.  No counterpart in the reference, whose cache
+ * is one sequence's f16 rows.
+ *
+ * Cache: K and V are n_pages pages of sinter_kv4_page_bytes each.  In a page,
+ * kv head after kv head: page_rows rows of hd / 2 code bytes (byte 16 b + i of
+ * a row: element 32 b + i in the low, 32 b + 16 + i in the high four bits),
+ * then page_rows rows of hd / 32 f16 scales, one per 32 elements.  An element
+ * is scale * (code - 8): the values of ggml's Q4_0.
+ *
+ * Batch: sequence s's new tokens are rows [tok_start[s], tok_start[s + 1]) of
+ * the token arrays (tok_start[0] = 0, never falling) and the last of the
+ * kv_len[s] rows it has: token i of n stands at position kv_len[s] - n + i.
+ * Its row r lies in page pages[s * max_pages + r / page_rows], at row r %
+ * page_rows.  All of tok_start, kv_len and pages is device memory, read by the
+ * kernels: a captured graph follows their values from replay to replay.
+ * Tokens at or behind tok_start[n_seq] are nobody's, and a token at a negative
+ * position has no row: the calls leave their outputs as they are (attention
+ * writes zeros for the latter).  Two tokens of one call must not share a row.
+ * A page number outside [0, n_pages), or a row past the table, raises
+ * SINTER_E_BAD_SHAPE (sinter_op_error; aux = the sequence): nothing is read or
+ * written there, and attention takes the rows for absent.
+ *
+ * Token arrays are F32, F16 or BF16 (`type`, the same for all of a call):
+ * element e of head h of token t at p[t * ld + h * hs + e], p 16-byte aligned,
+ * ld and hs multiples of 16 bytes.  Each call runs on the current device and
+ * only launches kernels on `stream`: none allocates, copies or waits, so all
+ * may be captured.  n_seq == 0 or n_tok == 0 is a no-op. */
+typedef struct sinter_heads {
+    void *p;
+    int64_t ld, hs;   /* elements from token to token, from head to head */
+} sinter_heads;
+
+typedef struct sinter_kv4_batch {
+    const int32_t *tok_start;  /* [n_seq + 1] */
+    const int32_t *kv_len;     /* [n_seq] rows, this call's tokens among them */
+    const int32_t *pages;      /* [n_seq][max_pages] */
+    void *kc, *vc;             /* 16-byte aligned */
+    uint32_t n_seq, n_tok;     /* n_tok: rows of the token arrays */
+    uint32_t max_pages, n_pages;
+    uint32_t page_rows;        /* a power of two, 16..2^20 */
+    uint32_t nkv, hd;          /* hd 64, 128 or 256 */
+    uint32_t _pad;
+} sinter_kv4_batch;
+
+/* bytes of one page of K (or of V); 0 for sizes that are not supported */
+size_t sinter_kv4_page_bytes(uint32_t page_rows, uint32_t nkv, uint32_t hd);
+
+/* q and k at their tokens' positions: per head y = x / sqrt(mean(x^2) + eps) *
+ * w (w f32 [hd], 16-byte aligned, null for none), then the pairs (i, i +
+ * rope_dims / 2) turned by pos * rope_base^(-2 i / rope_dims), the angle in
+ * fp64 (the decode instruction's is an fp32 product: at far positions the two
+ * differ by that rounding).  q and q_out (nq heads) or k and k_out (nkv heads)
+ * may be left out (null); an output may be its input.  The batch's cache
+ * fields are not read. */
+typedef struct sinter_kv4_prep_args {
+    sinter_heads q, q_out, k, k_out;
+    const float *q_norm, *k_norm;
+    uint32_t nq;
+    uint32_t rope_dims;   /* a multiple of 8, at most hd; 0: no rotation */
+    float rope_base, eps;
+    uint32_t type, _pad;
+} sinter_kv4_prep_args;
+int sinter_kv4_prep(const sinter_kv4_batch *b, const sinter_kv4_prep_args *a, void *stream);
+
+/* The tokens' k and v rows (nkv heads) quantised into their cache rows: per 32
+ * elements m = the first of the largest magnitude, d = m / -8, code = min(15,
+ * trunc(x * (1 / d) + 8.5)) in fp32, the scale f16(d) (ggml's
+ * quantize_row_q4_0_ref).  Magnitudes saturate at 65504; a NaN makes its
+ * block's scale NaN; a scale that rounds to 0 makes the block 0. */
+int sinter_kv4_append(const sinter_kv4_batch *b, const sinter_heads *k, const sinter_heads *v, int type, void *stream);
+
+/* The tokens' cache rows back as values, rounded once to `type`: all of a
+ * sequence with tok_start spanning its kv_len rows.  k or v may be null. */
+int sinter_kv4_read(const sinter_kv4_batch *b, const sinter_heads *k, const sinter_heads *v, int type, void *stream);
+
+/* Causal attention over the cache (its new rows appended before): the token at
+ * position p, q head h, gets sum_j softmax_j(scale q . k_j) v_j over rows j <=
+ * p of kv head h / (nq / nkv), times sigmoid(gate) where gate.p is not null;
+ * zeros if it sees no row.  fp32 scores, statistics and sums; q and the
+ * weights enter the matrix cores as f16 (two f16 parts, 22 bits, for F32).
+ * max_q and max_kv bound the new tokens and the rows of every sequence (a
+ * sequence over them raises SINTER_E_BAD_SHAPE); ws: sinter_kv4_attn_ws_bytes
+ * of device memory, 16-byte aligned (null if 0), used only while the call
+ * runs: calls that may overlap need one each. */
+typedef struct sinter_kv4_attn_args {
+    sinter_heads q, gate, out;   /* nq heads each */
+    void *ws;
+    size_t ws_bytes;
+    uint32_t nq, max_q, max_kv;
+    float scale;
+    uint32_t type, _pad;
+} sinter_kv4_attn_args;
+size_t sinter_kv4_attn_ws_bytes(const sinter_kv4_batch *b, const sinter_kv4_attn_args *a);
+int sinter_kv4_attn(const sinter_kv4_batch *b, const sinter_kv4_attn_args *a, void *stream);
+
 /* ------------------------------------------------------------------ synthetic data */
 /* Deterministic synthetic tensors (integer hashing plus exactly rounded fp32
  * arithmetic, so host and device produce identical bytes).  kind selects the

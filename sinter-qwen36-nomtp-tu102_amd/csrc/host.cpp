@@ -453,8 +453,10 @@ int sinter_op_error(uint32_t *code, uint32_t *aux) {
     unsigned h[2] = {0, 0};
     if (!hip_ok(hipMemcpy(h, err, 8, hipMemcpyDeviceToHost), "error cell read")) return SINTER_ERR_HIP;
     if (!hip_ok(hipMemset(err, 0, 8), "error cell clear")) return SINTER_ERR_HIP;
-    // the no-allocation op's cell on this device, when it has run here
-    if (unsigned *e2 = noalloc_err_cell()) {
+    // the no-allocation op's cell on this device, when it has run here, and
+    // the 4-bit KV cache's
+    for (unsigned *e2 : {noalloc_err_cell(), kv4_err_cell()}) {
+        if (!e2) continue;
         unsigned h2[2] = {0, 0};
         const unsigned zero[2] = {0, 0};
         if (!hip_ok(hipMemcpy(h2, e2, 8, hipMemcpyDeviceToHost), "error cell read") ||

@@ -92,8 +92,31 @@ class ModelConfig(C.Structure):
                 ("attn_chunks", C.c_int32), ("attn_chunk_min", C.c_int32)]
 
 
+class Heads(C.Structure):
+    _fields_ = [("p", vp), ("ld", C.c_int64), ("hs", C.c_int64)]
+
+
+class Kv4Batch(C.Structure):
+    _fields_ = [("tok_start", vp), ("kv_len", vp), ("pages", vp), ("kc", vp), ("vc", vp), ("n_seq", C.c_uint32),
+                ("n_tok", C.c_uint32), ("max_pages", C.c_uint32), ("n_pages", C.c_uint32), ("page_rows", C.c_uint32),
+                ("nkv", C.c_uint32), ("hd", C.c_uint32), ("_pad", C.c_uint32)]
+
+
+class Kv4PrepArgs(C.Structure):
+    _fields_ = [("q", Heads), ("q_out", Heads), ("k", Heads), ("k_out", Heads), ("q_norm", vp), ("k_norm", vp),
+                ("nq", C.c_uint32), ("rope_dims", C.c_uint32), ("rope_base", C.c_float), ("eps", C.c_float),
+                ("type", C.c_uint32), ("_pad", C.c_uint32)]
+
+
+class Kv4AttnArgs(C.Structure):
+    _fields_ = [("q", Heads), ("gate", Heads), ("out", Heads), ("ws", vp), ("ws_bytes", C.c_size_t),
+                ("nq", C.c_uint32), ("max_q", C.c_uint32), ("max_kv", C.c_uint32), ("scale", C.c_float),
+                ("type", C.c_uint32), ("_pad", C.c_uint32)]
+
+
 assert C.sizeof(Instr) == 256 and C.sizeof(GemvSeg) == 40
 assert C.sizeof(GemvArgs) == 224 and C.sizeof(GdnArgs) == 80 and C.sizeof(AttnArgs) == 136
+assert C.sizeof(Kv4Batch) == 72 and C.sizeof(Kv4PrepArgs) == 136 and C.sizeof(Kv4AttnArgs) == 112
 
 
 def qwen36_27b_config(n_ctx=4352, quant="q4_k_m", n_layer=64, kv="f16"):
@@ -167,6 +190,12 @@ def lib():
         "sinter_gated_rmsnorm_quant_q8k_ubatch": (I, [vp, vp, vp, U32, C.c_float, I64, U32, vp, vp]),
         "sinter_conv_silu_ubatch": (I, [vp, vp, vp, vp, I64, U32, U32, vp]),
         "sinter_op_attn_decode_noalloc": (I, [C.POINTER(AttnArgs), U32, vp]),
+        "sinter_kv4_page_bytes": (C.c_size_t, [U32, U32, U32]),
+        "sinter_kv4_prep": (I, [C.POINTER(Kv4Batch), C.POINTER(Kv4PrepArgs), vp]),
+        "sinter_kv4_append": (I, [C.POINTER(Kv4Batch), C.POINTER(Heads), C.POINTER(Heads), I, vp]),
+        "sinter_kv4_read": (I, [C.POINTER(Kv4Batch), C.POINTER(Heads), C.POINTER(Heads), I, vp]),
+        "sinter_kv4_attn_ws_bytes": (C.c_size_t, [C.POINTER(Kv4Batch), C.POINTER(Kv4AttnArgs)]),
+        "sinter_kv4_attn": (I, [C.POINTER(Kv4Batch), C.POINTER(Kv4AttnArgs), vp]),
         "sinter_litmus_barrier": (I, [U32, U32, I, C.POINTER(C.c_uint64)]),
         "sinter_copy_calibration": (I, [I, C.c_size_t, I]),
         "sinter_hbm_peak": (I, [C.c_uint64, U32, C.POINTER(C.c_double), C.POINTER(C.c_double)]),
