@@ -6,7 +6,9 @@
 //   kv4_append_kernel  k, v rows quantised into the cache's pages
 //   kv4_read_kernel    cache rows back to f32 / f16 / bf16
 //   kv4_split_kernel   attention of 16 (token, head) rows over a chunk of cache rows
-//   kv4_merge_kernel   the chunks' partials of a row joined
+//   kv4_merge_kernel   its chunks' partials of a row joined
+//   kv4_tile_kernel    attention of 128 rows of one sequence over a chunk
+//   kv4_join_kernel    its chunks' partials joined
 //
 // A page holds per kv head page_rows rows of codes (hd / 2 bytes; byte 16 b +
 // i of a row holds elements 32 b + i and 32 b + 16 + i in its low and high
@@ -29,6 +31,8 @@ namespace {
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef int i32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ f16x2 pair_of(uint32_t w) { return __builtin_bit_cast(f16x2, w); }
+typedef uint16_t __attribute__((may_alias)) u16a;   // (written as halves, read as wider words)
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float F16_MAX = 65504.0f;
@@ -268,60 +272,58 @@ struct Attn {
     sinter_heads q, gate, out;
     float *part;     // [slot][kv head][row tile][16][hd] unnormalised sums
     float2 *ml;      // [slot][kv head][row tile][16] reference and weight sum
+    float *tpart;    // kv4_tile_kernel's: [tile][kv head][chunk][tile rows][hd]
+    float2 *tml;
     uint32_t nq, gqa, max_q, max_kv, n_slots, n_mt, type, page_shift;
+    uint32_t n_tile, n_split, report;   // kv4_tile_kernel: row tiles and chunks; report the errors of lengths
+    uint32_t split_rows;   // sequences of up to these rows are kv4_split_kernel's (SPLIT_ROWS; 0: it is not launched)
     float qscale;    // scale * log2(e)
 };
 
+// The sequences of a call go two ways by their rows, (token, q head of a kv
+// head) pairs: up to SPLIT_ROWS of them to kv4_split_kernel, which streams the
+// cache past 16 rows, more to kv4_tile_kernel, whose waves share a tile's codes
+// once unpacked.
+constexpr uint32_t SPLIT_ROWS = 32;
+
 struct Work {
     int seq, len, tok0, n_new;   // the sequence: rows, first token, tokens (seq < 0: none)
-    uint32_t chunk, first, ct;   // the chunk of it, the slot of its chunk 0, tiles a chunk
+    uint32_t item, first;        // the item of it, the number of its item 0
 };
 
-// The chunks of all sequences lie in slots one after the other: ct tiles each,
-// the smallest ct for which they fit the launch's slots (sum of ceil(tiles /
-// ct) <= tiles / (n_slots - n_seq) + n_seq); a sequence with tokens has at
-// least one.  Finds slot `slot`'s work, or (by_seq) sequence `slot`'s first.
-__device__ __forceinline__ Work find_work(const Attn &a, uint32_t slot, bool by_seq, bool report) {
+// the most rows of a sequence that the launch and the page table have room for
+__device__ __forceinline__ uint32_t row_cap(const Attn &a) {
+    return (uint32_t)min((uint64_t)a.max_kv, (uint64_t)a.b.max_pages << a.page_shift);
+}
+
+// sequence base + lane: its rows, first token and tokens (0: none, or none of
+// them within the arrays).  report: raise the error of lengths over the bounds
+__device__ __forceinline__ void load_seq(const Attn &a, uint32_t base, bool report, int &len, int &t0, int &n) {
+    const uint32_t s = base + (threadIdx.x & 63u), i = min(s, a.b.n_seq - 1u);
+    t0 = a.b.tok_start[i];
+    n = a.b.tok_start[i + 1] - t0;
+    len = a.b.kv_len[i];
+    if (s >= a.b.n_seq) n = 0;
+    if (report && n > 0 && (len < 0 || (uint32_t)len > row_cap(a) || (uint32_t)n > a.max_q || t0 < 0 ||
+                            (uint32_t)t0 + (uint32_t)n > a.b.n_tok))
+        raise_error(g_kv4_err, SINTER_E_BAD_SHAPE, s);
+    if (t0 < 0 || n <= 0 || (uint32_t)t0 >= a.b.n_tok) n = 0;
+    else n = min(n, (int)(a.b.n_tok - (uint32_t)t0));
+    len = max(0, len);
+}
+
+// The sequences' items, count(len, n) each, numbered one sequence after the
+// other: item `id`'s sequence, or (by_seq) sequence `id` with its item 0.
+template <class Count>
+__device__ __forceinline__ Work locate(const Attn &a, uint32_t id, bool by_seq, bool report, Count count) {
     const uint32_t lane = threadIdx.x & 63u;
-    const sinter_kv4_batch &b = a.b;
-    auto load = [&](uint32_t base, int &len, int &t0, int &n) {
-        const uint32_t i = min(base + lane, b.n_seq - 1u);
-        t0 = b.tok_start[i];
-        n = b.tok_start[i + 1] - t0;
-        len = b.kv_len[i];
-        if (base + lane >= b.n_seq) n = 0;
-        const uint32_t cap = (uint32_t)min((uint64_t)a.max_kv, (uint64_t)b.max_pages << a.page_shift);
-        if (report && n > 0 && (len < 0 || (uint32_t)len > cap || (uint32_t)n > a.max_q || t0 < 0 || (uint32_t)(t0 + n) > b.n_tok))
-            raise_error(g_kv4_err, SINTER_E_BAD_SHAPE, base + lane);
-        // (tokens outside the arrays are nobody's)
-        if (t0 < 0 || n <= 0 || (uint32_t)t0 >= b.n_tok) n = 0;
-        else n = min(n, (int)(b.n_tok - (uint32_t)t0));
-        len = max(0, len);
-    };
-    auto tiles_of = [&](int len, int n) {
-        const uint32_t cap = (uint32_t)min((uint64_t)a.max_kv, (uint64_t)b.max_pages << a.page_shift);
-        return n > 0 ? max(1u, (min((uint32_t)len, cap) + TILE - 1u) / TILE) : 0u;
-    };
-    int len, t0, n;
-    uint32_t total = 0;
-    for (uint32_t base = 0; base < b.n_seq; base += 64) {
-        load(base, len, t0, n);
-        uint32_t v = tiles_of(len, n);
-        v += (uint32_t)dpp_i<DPP_XOR1>((int)v);
-        v += (uint32_t)dpp_i<DPP_XOR2>((int)v);
-        v += (uint32_t)dpp_i<DPP_HALF_MIRROR>((int)v);
-        v += (uint32_t)dpp_i<DPP_MIRROR>((int)v);
-#pragma unroll
-        for (int r = 0; r < 4; r++) total += (uint32_t)__builtin_amdgcn_readlane((int)v, 16 * r);
-    }
-    const uint32_t room = a.n_slots - b.n_seq;
     Work w;
     w.seq = -1;
-    w.ct = max(CT_MIN, room ? (total + room - 1u) / room : 0x7fffffu);
     uint32_t before = 0;
-    for (uint32_t base = 0; base < b.n_seq; base += 64) {
-        if (b.n_seq > 64) load(base, len, t0, n);
-        const uint32_t c = n > 0 ? (tiles_of(len, n) + w.ct - 1u) / w.ct : 0u;
+    for (uint32_t base = 0; base < a.b.n_seq; base += 64) {
+        int len, t0, n;
+        load_seq(a, base, report, len, t0, n);
+        const uint32_t c = n > 0 ? count(len, n) : 0u;
         uint32_t sum = c;   // inclusive over the lanes
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -329,21 +331,61 @@ __device__ __forceinline__ Work find_work(const Attn &a, uint32_t slot, bool by_
             if (lane >= (uint32_t)o) sum += p;
         }
         const uint32_t lo = before + sum - c;
-        const bool mine = by_seq ? base + lane == slot && n > 0 : slot >= lo && slot < lo + c;
+        const bool mine = c > 0 && (by_seq ? base + lane == id : id >= lo && id < lo + c);
         const uint64_t m = __builtin_amdgcn_ballot_w64(mine);
-        if (m != 0) {
+        if (m != 0 && w.seq < 0) {
             const int l = __builtin_ctzll(m);
             w.seq = (int)base + l;
             w.len = __builtin_amdgcn_readlane(len, l);
             w.tok0 = __builtin_amdgcn_readlane(t0, l);
             w.n_new = __builtin_amdgcn_readlane(n, l);
             w.first = (uint32_t)__builtin_amdgcn_readlane((int)lo, l);
-            w.chunk = by_seq ? 0u : slot - w.first;
-            return w;
+            w.item = by_seq ? 0u : id - w.first;
+            if (!report) return w;
         }
         before += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
     }
     return w;
+}
+
+__device__ __forceinline__ bool is_split(const Attn &a, int n) { return (uint32_t)n * a.gqa <= a.split_rows; }
+
+// kv4_split_kernel's chunks: ct tiles of rows each, the smallest ct for which
+// all of them fit the launch's slots (sum of ceil(tiles / ct) <= tiles /
+// (n_slots - n_seq) + n_seq); a sequence with tokens has at least one.
+__device__ __forceinline__ uint32_t tiles_of(const Attn &a, int len, int n) {
+    return is_split(a, n) ? max(1u, (min((uint32_t)len, row_cap(a)) + TILE - 1u) / TILE) : 0u;
+}
+__device__ __forceinline__ uint32_t chunk_tiles(const Attn &a) {
+    uint32_t total = 0;
+    for (uint32_t base = 0; base < a.b.n_seq; base += 64) {
+        int len, t0, n;
+        load_seq(a, base, false, len, t0, n);
+        uint32_t v = n > 0 ? tiles_of(a, len, n) : 0u;
+        v += (uint32_t)dpp_i<DPP_XOR1>((int)v);
+        v += (uint32_t)dpp_i<DPP_XOR2>((int)v);
+        v += (uint32_t)dpp_i<DPP_HALF_MIRROR>((int)v);
+        v += (uint32_t)dpp_i<DPP_MIRROR>((int)v);
+#pragma unroll
+        for (int r = 0; r < 4; r++) total += (uint32_t)__builtin_amdgcn_readlane((int)v, 16 * r);
+    }
+    const uint32_t room = a.n_slots - a.b.n_seq;
+    return max(CT_MIN, room ? (total + room - 1u) / room : 0x7fffffu);
+}
+__device__ __forceinline__ Work find_chunk(const Attn &a, uint32_t ct, uint32_t id, bool by_seq, bool report) {
+    return locate(a, id, by_seq, report, [&](int len, int n) { return (tiles_of(a, len, n) + ct - 1u) / ct; });
+}
+
+// the gated, normalised output of four elements
+__device__ __forceinline__ void store_out(const Attn &a, int64_t t, int64_t h, uint32_t e, f32x4 o, float l) {
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+    float4 y = make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+    if (a.gate.p) {
+        const float4 z = load4(a.gate.p, t * a.gate.ld + h * a.gate.hs + e, a.type);
+        auto sig = [](float x) { return 1.0f / (1.0f + __builtin_amdgcn_exp2f(x * -1.44269504088896341f)); };
+        y = make_float4(y.x * sig(z.x), y.y * sig(z.y), y.z * sig(z.z), y.w * sig(z.w));
+    }
+    store4(a.out.p, t * a.out.ld + h * a.out.hs + e, a.type, y);
 }
 
 // one LDS-DMA of 16 bytes a lane from per-lane addresses (lane l's land at lds_base + 16 l)
@@ -405,17 +447,18 @@ __global__ __launch_bounds__(256, 2) void kv4_split_kernel(Attn a) {
     const uint32_t r16 = lane & 15u, g4 = lane >> 4, NKV = a.b.nkv;
     const uint32_t per = a.n_slots * NKV, mt = blockIdx.x / per, it = blockIdx.x % per;
     const uint32_t g = it % NKV, slot = it / NKV;
-    const Work wk = find_work(a, slot, false, it == 0 && mt == 0 && w == 0);
+    const uint32_t ct = chunk_tiles(a);
+    const Work wk = find_chunk(a, ct, slot, false, blockIdx.x == 0 && w == 0);
     if (wk.seq < 0) return;
     const uint32_t M = (uint32_t)wk.n_new * a.gqa;
     if (16 * mt >= M) return;
     const uint32_t rows = min(16u, M - 16 * mt);
     const int p0 = wk.len - wk.n_new;   // the first token's position
     auto row_pos = [&](uint32_t r) { return p0 + (int)((16 * mt + r) / a.gqa); };
-    const int pmin = row_pos(0), pmax = row_pos(rows - 1), c0 = (int)(wk.chunk * wk.ct * TILE);
-    if (wk.chunk > 0 && c0 > pmax) return;
-    const int cap = (int)min((uint64_t)a.max_kv, (uint64_t)a.b.max_pages << a.page_shift);
-    const int end = min(min(c0 + (int)(wk.ct * TILE), pmax + 1), cap);   // rows [c0, end)
+    const int pmin = row_pos(0), pmax = row_pos(rows - 1), c0 = (int)(wk.item * ct * TILE);
+    if (wk.item > 0 && c0 > pmax) return;
+    const int cap = (int)row_cap(a);
+    const int end = min(min(c0 + (int)(ct * TILE), pmax + 1), cap);   // rows [c0, end)
     const int my_vis = r16 < rows ? min(row_pos(r16) + 1, end) : end;     // of them this lane's row sees [c0, my_vis)
     const int n_tile = end > c0 ? (end - c0 + (int)TILE - 1) / (int)TILE : 0;
 
@@ -572,7 +615,7 @@ __global__ __launch_bounds__(256, 2) void kv4_split_kernel(Attn a) {
                 if constexpr (NS == 2) t = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, Q[NS - 1][b], t, 0, 0, 0);
 #pragma unroll
                 for (uint32_t v = 0; v < 4; v++) {
-                    const f16x2 dd = __builtin_bit_cast(f16x2, d[v][b / 2]);
+                    const f16x2 dd = pair_of(d[v][b / 2]);
                     s[h][v] = fmaf(t[v], (float)(b & 1 ? dd.y : dd.x), s[h][v]);
                 }
             }
@@ -655,7 +698,7 @@ __global__ __launch_bounds__(256, 2) void kv4_split_kernel(Attn a) {
 #pragma unroll
             for (uint32_t k = 0; k < 8; k++) {
                 const uint32_t key = (k & 4) | ((k & 1) << 1) | ((k >> 1) & 1);   // 0 2 1 3 4 6 5 7
-                const f16x2 dd = __builtin_bit_cast(f16x2, dv[key][b / 2]);
+                const f16x2 dd = pair_of(dv[key][b / 2]);
                 const float dk = (float)(b & 1 ? dd.y : dd.x);
                 if constexpr (NS == 1) {
                     P[k] = (_Float16)fmaf(p[key], dk, 0.0f);
@@ -704,17 +747,9 @@ __global__ __launch_bounds__(256, 2) void kv4_split_kernel(Attn a) {
             for (int j = 0; j < 4; j++) o[j] = fmaf(x[j], c, o[j]);
         }
         const int pos = min(row_pos(r), cap - 1);   // (cap: rows the launch and the table have room for)
-        if (pos < c0 && wk.chunk > 0) continue;   // (the row ends before this chunk)
-        if (pos < (int)(wk.ct * TILE)) {   // the row sees chunk 0 alone
-            const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-            const int64_t t = wk.tok0 + (int)((16 * mt + r) / a.gqa), h = g * a.gqa + (16 * mt + r) % a.gqa;
-            float4 y = make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-            if (a.gate.p) {
-                const float4 z = load4(a.gate.p, t * a.gate.ld + h * a.gate.hs + e, a.type);
-                auto sig = [](float x) { return 1.0f / (1.0f + __builtin_amdgcn_exp2f(x * -1.44269504088896341f)); };
-                y = make_float4(y.x * sig(z.x), y.y * sig(z.y), y.z * sig(z.z), y.w * sig(z.w));
-            }
-            store4(a.out.p, t * a.out.ld + h * a.out.hs + e, a.type, y);
+        if (pos < c0 && wk.item > 0) continue;   // (the row ends before this chunk)
+        if (pos < (int)(ct * TILE)) {   // the row sees chunk 0 alone
+            store_out(a, wk.tok0 + (int)((16 * mt + r) / a.gqa), g * a.gqa + (16 * mt + r) % a.gqa, e, o, l);
         } else {
             const size_t rec = (((size_t)slot * NKV + g) * a.n_mt + mt) * 16 + r;
             *reinterpret_cast<f32x4 *>(a.part + rec * HD + e) = o;
@@ -724,23 +759,20 @@ __global__ __launch_bounds__(256, 2) void kv4_split_kernel(Attn a) {
 }
 
 // A row that sees more than one chunk: out = sum c_i O_i / sum c_i l_i with
-// c_i = exp2(ref_i - max ref).  One workgroup per (token, q head); wave w takes
-// every fourth chunk.
-__global__ __launch_bounds__(256) void kv4_merge_kernel(Attn a) {
+// c_i = exp2(ref_i - max ref).  One workgroup per (sequence, kv head, row);
+// wave w takes every fourth chunk.
+__global__ __launch_bounds__(256) void kv4_merge_kernel(Attn a, uint32_t rows) {
     __shared__ float red[2][4];
     __shared__ __attribute__((aligned(16))) float comb[4][256];
-    const uint32_t t = blockIdx.x / a.nq, h = blockIdx.x % a.nq, lane = threadIdx.x & 63u, HD = a.b.hd;
+    const uint32_t r = blockIdx.x % rows, sg = blockIdx.x / rows, g = sg % a.b.nkv, lane = threadIdx.x & 63u, HD = a.b.hd;
     const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int seq = seq_of(a.b, t);
-    if (seq < 0) return;
-    const Work wk = find_work(a, (uint32_t)seq, true, false);
+    const uint32_t ct = chunk_tiles(a);
+    const Work wk = find_chunk(a, ct, sg / a.b.nkv, true, false);
     if (wk.seq < 0) return;
-    const uint32_t i = t - (uint32_t)wk.tok0, span = wk.ct * TILE;
-    const int cap = (int)min((uint64_t)a.max_kv, (uint64_t)a.b.max_pages << a.page_shift);
-    const int pos = min(wk.len - wk.n_new + (int)i, cap - 1);
-    if (i >= (uint32_t)wk.n_new || i >= a.max_q || pos < (int)span) return;
+    const uint32_t i = r / a.gqa, h = g * a.gqa + r % a.gqa, t = (uint32_t)wk.tok0 + i, span = ct * TILE;
+    const int pos = min(wk.len - wk.n_new + (int)i, (int)row_cap(a) - 1);
+    if (i >= (uint32_t)wk.n_new || pos < (int)span) return;
     const uint32_t n = (uint32_t)pos / span + 1u;   // chunks the row sees
-    const uint32_t g = h / a.gqa, r = i * a.gqa + h % a.gqa;
     auto rec = [&](uint32_t c) { return (((size_t)(wk.first + c) * a.b.nkv + g) * a.n_mt + r / 16) * 16 + r % 16; };
     float m = REF_NONE, l = 0.0f;
     for (uint32_t c = lane; c < n; c += 64) m = fmaxf(m, a.ml[rec(c)].x);
@@ -772,14 +804,528 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(Attn a) {
     l = (red[0][0] + red[0][1]) + (red[0][2] + red[0][3]);
 #pragma unroll
     for (uint32_t k = 1; k < 4; k++) o = o + *reinterpret_cast<const f32x4 *>(&comb[k][e]);
-    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-    float4 y = make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-    if (a.gate.p) {
-        const float4 z = load4(a.gate.p, (int64_t)t * a.gate.ld + (int64_t)h * a.gate.hs + e, a.type);
-        auto sig = [](float x) { return 1.0f / (1.0f + __builtin_amdgcn_exp2f(x * -1.44269504088896341f)); };
-        y = make_float4(y.x * sig(z.x), y.y * sig(z.y), y.z * sig(z.z), y.w * sig(z.w));
+    store_out(a, t, h, e, o, l);
+}
+
+// ------------------------------------------------------------------ many rows
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// the tiles of ROWS rows of sequences that kv4_split_kernel leaves out
+__device__ __forceinline__ Work find_tile(const Attn &a, uint32_t rows, uint32_t id, bool by_seq, bool report) {
+    return locate(a, id, by_seq, report, [&](int len, int n) {
+        return is_split(a, n) ? 0u : ((uint32_t)n * a.gqa + rows - 1u) / rows;
+    });
+}
+__device__ __forceinline__ uint32_t wave_sum_u32(uint32_t v) {
+    v += (uint32_t)dpp_i<DPP_XOR1>((int)v);
+    v += (uint32_t)dpp_i<DPP_XOR2>((int)v);
+    v += (uint32_t)dpp_i<DPP_HALF_MIRROR>((int)v);
+    v += (uint32_t)dpp_i<DPP_MIRROR>((int)v);
+    uint32_t t = 0;
+#pragma unroll
+    for (int r = 0; r < 4; r++) t += (uint32_t)__builtin_amdgcn_readlane((int)v, 16 * r);
+    return t;
+}
+// The id-th tile from the one with the most cache rows down, so that the
+// longest start first (two prompts of 2000 tokens, bf16, 27B heads: sequence
+// after sequence 377 us, so 205).  A sequence with p0 rows before its tokens
+// has one tile in each of the levels p0 gqa / rows + 0, 1, ..: the level is
+// found by bisection over the count of tiles at or above it, a lane a
+// sequence.  More than 64 sequences are taken in their order.
+__device__ __forceinline__ Work find_ranked_tile(const Attn &a, uint32_t rows, uint32_t id, bool report) {
+    if (a.b.n_seq > 64) return find_tile(a, rows, id, false, report);
+    int len, t0, n;
+    load_seq(a, 0, report, len, t0, n);
+    const uint32_t c = n > 0 && !is_split(a, n) ? ((uint32_t)n * a.gqa + rows - 1u) / rows : 0u;
+    const uint32_t base = (uint32_t)((uint64_t)(uint32_t)max(0, len - n) * a.gqa / rows), top = c ? base + c : 0u;
+    // (no branch on c: every lane takes part in the sums)
+    auto above = [&](uint32_t y) { return wave_sum_u32(min(c, max(top, y) - y)); };
+    Work w;
+    w.seq = -1;
+    if (above(0) <= id) return w;
+    // above(lo) > id >= above(hi)
+    uint32_t lo = 0, hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)wave_max_f32((float)top) + 1);
+    while (hi - lo > 1) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        if (above(mid) > id) lo = mid;
+        else hi = mid;
     }
-    store4(a.out.p, (int64_t)t * a.out.ld + (int64_t)h * a.out.hs + e, a.type, y);
+    const bool in = lo >= base && lo < top;
+    const uint64_t all = __builtin_amdgcn_ballot_w64(in);
+    const uint32_t before = __builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0u));
+    const uint32_t rank = id - above(hi);
+    const uint64_t m = __builtin_amdgcn_ballot_w64(in && before == rank);
+    if (m == 0) return w;
+    const int l = __builtin_ctzll(m);
+    w.seq = l;
+    w.len = __builtin_amdgcn_readlane(len, l);
+    w.tok0 = __builtin_amdgcn_readlane(t0, l);
+    w.n_new = __builtin_amdgcn_readlane(n, l);
+    w.item = lo - (uint32_t)__builtin_amdgcn_readlane((int)base, l);
+    // (the tiles of the sequences before it)
+    w.first = wave_sum_u32((threadIdx.x & 63u) < (uint32_t)l ? c : 0u);
+    return w;
+}
+// the cache rows a chunk of a tile that sees `seen` rows takes
+constexpr uint32_t CHUNK_MIN = 512;
+__device__ __forceinline__ uint32_t chunk_rows(uint32_t seen, uint32_t n_split) {
+    return max(CHUNK_MIN, ((seen + n_split - 1u) / n_split + TILE - 1u) / TILE * TILE);
+}
+
+// Work item: (tile of 32 NW rows, kv head, chunk of the cache rows the tile
+// sees); wave w has rows 32 w .. 32 w + 31.  The waves unpack each 32-row cache
+// tile into LDS together, a tile ahead of its use, so that its codes are taken
+// apart once for 32 NW rows:
+//   K  fragments [16-dim slice][half][32 keys] of 8 dims: the exact codes, the
+//      scales multiplying each block's fp32 sum (KX), or, for BF16 rows,
+//      f16(scale * code): 2^-12 of an element, well under the output's 2^-9
+//   V  fragments [32-dim block][8-key group][32 dims] of 8 keys, transposed by
+//      the LDS read of the raw codes: f16(scale * code), for F32 a second
+//      fragment holds the rest of it (scale * code has 15 bits: exact in two)
+// The weights are one f16 for BF16 rows and two (NP) for F16 and F32: with the
+// rounded V one f16 would put F16 results at 1.6 times the error that rounding
+// them once has, two at 1.26.
+// Every operand read is 1 KiB of consecutive LDS.  Scores S^T = K Q^T and sums
+// O^T = V^T P^T run on 32x32x16 f16 MFMA: D holds key 8 i + 4 (l / 32) + j of
+// row l % 32 in lane l, the B operand's layout of P^T with the keys of a group
+// in that order, so P stays in its lane.  The weights' reference moves as in
+// kv4_split_kernel (with no scale in it: p <= 2^TOP).
+//
+// A V scale that is not finite would reach rows that do not see its key (0
+// times it): it is 0 in the fragments and named in `odd`, and makes NaN of the
+// block's sums of the rows that do.
+template <int HD, int T, int NW>
+__global__ __launch_bounds__(64 * NW, T == SINTER_F32 ? 1 : 2) void kv4_tile_kernel(Attn a) {
+    constexpr uint32_t NS = T == SINTER_F32 ? 2 : 1, NP = T == SINTER_BF16 ? 1 : 2;   // f16 parts of q (and V), of the weights
+    constexpr bool KX = T != SINTER_BF16;
+    constexpr uint32_t NB = HD / 32, HB = HD / 2, SB = HD / 16, NCH = HB / 16, KC = TILE * HB, ROWS = 32 * NW;
+    constexpr uint32_t SH = HD == 256 ? 1 : HD == 128 ? 2 : 3, BPW = NB > NW ? NB / NW : 1, ACT = NB / BPW;
+    constexpr uint32_t KF = NB * 2048, VF = NB * 2048, KS = KX ? NB * 64 : 0, BUF = KF + NS * VF + KS;
+    // (the output's passes: blocks of 32 dims a pass, 16-byte units a row, bytes a wave)
+    constexpr uint32_t FIT = 2 * BUF / (NW * 4096), PB = FIT >= 4 && NB >= 4 ? 4 : FIT >= 2 ? 2 : 1, UN = PB * 8, PASS = PB * 4096;
+    __shared__ __attribute__((aligned(16))) unsigned char frag[2 * BUF > NW * PASS ? 2 * BUF : NW * PASS];
+    __shared__ __attribute__((aligned(16))) unsigned char raw[2 * KC];
+    __shared__ __attribute__((aligned(16))) _Float16 vsc[NB][32];
+    __shared__ __attribute__((aligned(16))) uint32_t odd[2][8];
+    // (F16 rows of 256: a block's sums beside the scores leave no registers
+    // for all of q, the last QL slices are read from LDS)
+    constexpr uint32_t QL = HD == 256 && KX && NS == 1 ? 4 : 0, QR = 2 * NB - QL;
+    __shared__ __attribute__((aligned(16))) f16x8 qx[QL ? NW * QL * 64 : 1];
+    const uint32_t lane = threadIdx.x & 63u, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t l32 = lane & 31u, hf = lane >> 5, NKV = a.b.nkv;
+    uint32_t id = blockIdx.x;
+    const uint32_t g = id % NKV;
+    id /= NKV;
+    const uint32_t ck = id / a.n_tile;
+    const Work wk = find_ranked_tile(a, ROWS, id % a.n_tile, a.report && blockIdx.x == 0 && w == 0);
+    if (wk.seq < 0) return;
+    const uint32_t gt = wk.first + wk.item;
+    const uint32_t M = (uint32_t)wk.n_new * a.gqa, r0 = wk.item * ROWS;
+    const int p0 = wk.len - wk.n_new, cap = (int)row_cap(a);
+    auto row_pos = [&](uint32_t r) { return p0 + (int)(min(r, M - 1u) / a.gqa); };
+    const int seen = max(0, min(row_pos(r0 + ROWS - 1u) + 1, cap));   // rows the tile's last row sees
+    const uint32_t per = chunk_rows((uint32_t)seen, a.n_split);
+    const int c0 = (int)(ck * per), end = min(seen, c0 + (int)per);   // rows [c0, end)
+    if (ck > 0 && c0 >= seen) return;
+    const bool whole = (uint32_t)seen <= per;   // one chunk
+    const int n_tile = end > c0 ? (end - c0 + (int)TILE - 1) / (int)TILE : 0;
+    const uint32_t row = r0 + 32 * w + l32;
+    const bool live = row < M;
+    const int my_vis = live ? min(row_pos(row) + 1, end) : end;
+    const int wmin = __builtin_amdgcn_readfirstlane(min(row_pos(r0 + 32 * w) + 1, end));        // the wave's first row's
+    const int wmax = r0 + 32 * w < M ? __builtin_amdgcn_readfirstlane(min(row_pos(r0 + 32 * w + 31u) + 1, end)) : 0;   // and last row's end
+
+    // q: slice m = 2 b + half holds dims 32 b + 16 half + 8 hf + {0 2 1 3 4 6 5 7} (the codes' order)
+    f16x8 Q[NS][2 * NB];
+    float qs;
+    {
+        const int64_t tok = wk.tok0 + (int)(min(row, M - 1u) / a.gqa), head = g * a.gqa + min(row, M - 1u) % a.gqa;
+        const int64_t e0 = tok * a.q.ld + head * a.q.hs + 8 * hf;
+        float am = 0.0f;
+        auto scale_of = [&](float m) {
+            m = fmaxf(m, __shfl_xor(m, 32, 64));
+            return m > 0.0f && m < INFINITY ? 14 - (int)((__float_as_uint(fmaxf(m, 1e-30f)) >> 23) - 126u) : 0;
+        };
+        if constexpr (NS == 2) {
+            const float *src = static_cast<const float *>(a.q.p) + e0;
+#pragma unroll
+            for (uint32_t m = 0; m < 2 * NB; m++)
+#pragma unroll
+                for (uint32_t k = 0; k < 8; k++) am = fmaxf(am, fabsf(src[16 * m + k]));
+            const int ex = scale_of(am);
+            const float up = live ? ldexpf(1.0f, ex) : 0.0f;
+            qs = a.qscale * ldexpf(1.0f, -ex);
+#pragma unroll
+            for (uint32_t m = 0; m < 2 * NB; m++) {
+                const float4 x = reinterpret_cast<const float4 *>(src + 16 * m)[0], y = reinterpret_cast<const float4 *>(src + 16 * m)[1];
+                float f[8] = {x.x * up, x.z * up, x.y * up, x.w * up, y.x * up, y.z * up, y.y * up, y.w * up};
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    asm volatile("" : "+v"(f[i]));   // (as for the weights in kv4_split_kernel)
+                    const _Float16 hi = (_Float16)f[i];
+                    Q[0][m][i] = hi;
+                    Q[NS - 1][m][i] = (_Float16)(f[i] - (float)hi);
+                }
+            }
+        } else {
+            u32x4 u[2 * NB];
+#pragma unroll
+            for (uint32_t m = 0; m < 2 * NB; m++)
+                u[m] = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.q.p) + e0 + 16 * m);
+            const bool bf = a.type == SINTER_BF16;
+            auto val = [&](uint32_t m, int k) {
+                const uint32_t x = u[m][k >> 1];
+                const float b = __uint_as_float(k & 1 ? x & 0xffff0000u : x << 16);
+                const float h = h2f((uint16_t)(k & 1 ? x >> 16 : x));
+                return bf ? b : h;
+            };
+#pragma unroll
+            for (uint32_t m = 0; m < 2 * NB; m++)
+#pragma unroll
+                for (int k = 0; k < 8; k++) am = fmaxf(am, fabsf(val(m, k)));
+            const int ex = scale_of(am);
+            const float up = live ? ldexpf(1.0f, ex) : 0.0f;
+            qs = a.qscale * ldexpf(1.0f, -ex);
+#pragma unroll
+            for (uint32_t m = 0; m < 2 * NB; m++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) Q[0][m][i] = (_Float16)(val(m, (i & 4) | ((i & 1) << 1) | ((i >> 1) & 1)) * up);
+        }
+    }
+
+    if constexpr (QL > 0) {
+#pragma unroll
+        for (uint32_t m = QR; m < 2 * NB; m++) qx[(w * QL + m - QR) * 64 + lane] = Q[0][m];
+    }
+
+    // --- a cache tile's way in: loads (two tiles ahead), unpacking (one ahead)
+    const size_t head_bytes = ((size_t)HB + SB) << a.page_shift, page_bytes = head_bytes * NKV;
+    const uint64_t kc = (uint64_t)a.b.kc + g * head_bytes, vc = (uint64_t)a.b.vc + g * head_bytes;
+    const uint32_t pmask = (1u << a.page_shift) - 1u;
+    auto swz = [](uint32_t r) { return ((r >> SH) ^ ((r >> 4) * (NCH / 2))) & (NCH - 1); };
+    const int32_t *table = a.b.pages + (size_t)wk.seq * a.b.max_pages;
+    uint32_t win = 0x80000000u;
+    int ids = 0;
+    auto page_at = [&](int r, uint32_t &holes, uint32_t half) -> uint32_t {
+        const uint32_t e = (uint32_t)r >> a.page_shift;
+        if (e - win >= 64u) {
+            win = e;
+            ids = table[min(e + lane, a.b.max_pages - 1u)];
+        }
+        const uint32_t p = (uint32_t)__builtin_amdgcn_readlane(ids, (int)(e - win));
+        if (p < a.b.n_pages) return p;
+        if (lane == 0) raise_error(g_kv4_err, SINTER_E_BAD_SHAPE, (unsigned)wk.seq);
+        holes |= half;
+        return 0;
+    };
+    const LDS unsigned char *R = (const LDS unsigned char *)raw;
+    const uint32_t rbase = (uint32_t)(uintptr_t)(LDS unsigned char *)raw;
+    LDS unsigned char *F = (LDS unsigned char *)frag;
+    struct In { u32x2 k[BPW]; uint32_t sc[BPW], holes; };   // (sc: K's scale, V's above it)
+    auto issue = [&](int j, In &in) {
+        uint32_t ln = lane;
+        asm volatile("" : "+v"(ln));   // (opaque: addresses made of it would be kept through the loop)
+        const uint32_t l32 = ln & 31u, hf = ln >> 5;
+        const int r = c0 + j * (int)TILE;
+        in.holes = 0;
+        const uint32_t in0 = (uint32_t)r & pmask, to = rbase + (j & 1) * KC;
+        const uint64_t o0 = page_at(r, in.holes, 1u) * page_bytes;
+        // V's codes to LDS, 1 KiB a wave; K's codes of the wave's blocks, both scales: key l32
+        auto load = [&](auto codes, auto scales) {
+            for (uint32_t i = w; i < KC / 1024; i += NW) {
+                const uint32_t u = 64 * i + ln, rr = u / NCH;
+                lds_dma16v((uint64_t)codes(vc, rr, 16 * ((u % NCH) ^ swz(rr))), to + 1024 * i);
+            }
+            if (ACT < NW && w >= ACT) return;
+            const GLB unsigned char *kp = codes(kc, l32, 16 * BPW * w + 8 * hf);
+            const GLB uint16_t *ksp = (const GLB uint16_t *)scales(kc, l32, 2 * BPW * w);
+            const GLB uint16_t *vsp = (const GLB uint16_t *)scales(vc, l32, 2 * BPW * w);
+#pragma unroll
+            for (uint32_t i = 0; i < BPW; i++) {
+                in.k[i] = *reinterpret_cast<const GLB u32x2 *>(kp + 16 * i);
+                in.sc[i] = (uint32_t)ksp[i] | ((uint32_t)vsp[i] << 16);
+            }
+        };
+        const uint64_t plane = (uint64_t)HB << a.page_shift;
+        if (a.page_shift >= 5) {   // a tile lies in one page: one address and a lane's offset
+            const uint64_t co = o0 + (uint64_t)in0 * HB, so = o0 + plane + (uint64_t)in0 * SB;
+            in.holes |= in.holes << 1;
+            load([&](uint64_t c, uint32_t rr, uint32_t off) { return (const GLB unsigned char *)(c + co) + (rr * HB + off); },
+                 [&](uint64_t c, uint32_t rr, uint32_t off) { return (const GLB unsigned char *)(c + so) + (rr * SB + off); });
+        } else {
+            uint64_t o1 = o0;   // (rows past the end: the first half's again, masked)
+            if (r + 16 < end) o1 = page_at(r + 16, in.holes, 2u) * page_bytes;
+            load([&](uint64_t c, uint32_t rr, uint32_t off) { return (const GLB unsigned char *)(c + (rr < 16 ? o0 : o1)) + ((rr & 15u) * HB + off); },
+                 [&](uint64_t c, uint32_t rr, uint32_t off) {
+                     return (const GLB unsigned char *)(c + (rr < 16 ? o0 : o1) + plane) + ((rr & 15u) * SB + off);
+                 });
+        }
+    };
+    auto unpack = [&](int j, const In &in) {
+        if (ACT < NW && w >= ACT) return;
+        uint32_t ln = lane;
+        asm volatile("" : "+v"(ln));   // (opaque, as in issue)
+        const uint32_t l32 = ln & 31u, hf = ln >> 5;
+        LDS unsigned char *B = F + (j & 1) * BUF;
+        const LDS unsigned char *V = R + (j & 1) * KC;
+        const bool real = c0 + j * (int)TILE + (int)l32 < end && !(in.holes >> (l32 >> 4) & 1u);
+        const uint32_t r16 = ln & 15u, g4 = ln >> 4;
+#pragma unroll
+        for (uint32_t i = 0; i < BPW; i++) {
+            const uint32_t b = BPW * w + i;
+            // V scales in the operand's key order (read back below by this wave alone): key 16 s + 4 h + x (x < 4), 8 + x (x >= 4) of group 2 s + h
+            const uint32_t vb = real ? in.sc[i] >> 16 : 0u;
+            const bool fin = (vb & 0x7c00u) != 0x7c00u;
+            const uint64_t bad = __builtin_amdgcn_ballot_w64(!fin);
+            if (ln == 0) odd[j & 1][b] = (uint32_t)bad;
+            {
+                const uint32_t grp = 2 * (l32 >> 4) + ((l32 >> 2) & 1u), x = (l32 & 3u) + ((l32 >> 1) & 4u);
+                const uint32_t at = (x & 4) | ((x & 1) << 1) | ((x >> 1) & 1);   // 0 2 1 3 4 6 5 7
+                ((LDS u16a *)vsc)[b * 32 + grp * 8 + at] = (uint16_t)(fin ? vb : 0u);
+            }
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < BPW; i++) {
+            const uint32_t b = BPW * w + i;
+            f16x2 kl[4] = {code_pair_lo(in.k[i].x), code_pair_lo(in.k[i].x >> 8), code_pair_lo(in.k[i].y), code_pair_lo(in.k[i].y >> 8)};
+            f16x2 kh[4] = {code_pair_hi(in.k[i].x), code_pair_hi(in.k[i].x >> 8), code_pair_hi(in.k[i].y), code_pair_hi(in.k[i].y >> 8)};
+            if constexpr (!KX) {
+                const _Float16 d = __builtin_bit_cast(_Float16, (uint16_t)(real ? in.sc[i] : 0u));
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    kl[c] = kl[c] * f16x2{d, d};
+                    kh[c] = kh[c] * f16x2{d, d};
+                }
+            } else if (hf == 0) {
+                ((LDS u16a *)(B + KF + NS * VF))[b * 32 + l32] = (uint16_t)(real ? in.sc[i] : 0u);
+            }
+            *reinterpret_cast<LDS f16x8 *>(B + (2 * b) * 1024 + 16 * ln) = join8(kl[0], kl[1], kl[2], kl[3]);
+            *reinterpret_cast<LDS f16x8 *>(B + (2 * b + 1) * 1024 + 16 * ln) = join8(kh[0], kh[1], kh[2], kh[3]);
+            // V: lane r16 of group g4 gets byte r16 of the group's eight keys
+            const uint32_t kr = r16 >> 1, vr = 16 * (g4 >> 1) + 4 * (g4 & 1u) + (kr & 3u) + 8 * (kr >> 2);
+            const i32x2 x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((LDS i32x2 *)(V + vr * HB + 16 * (b ^ swz(vr)) + 8 * (r16 & 1u)));
+            const u32x4 dp = *reinterpret_cast<const LDS u32x4 *>((const LDS uint16_t *)vsc + b * 32 + g4 * 8);
+            const uint32_t x0 = (uint32_t)x.x, x1 = (uint32_t)x.y;
+            const f16x2 vl[4] = {code_pair_lo(x0), code_pair_lo(x0 >> 8), code_pair_lo(x1), code_pair_lo(x1 >> 8)};
+            const f16x2 vh[4] = {code_pair_hi(x0), code_pair_hi(x0 >> 8), code_pair_hi(x1), code_pair_hi(x1 >> 8)};
+            f16x2 hl[4], hh[4];
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const f16x2 d = pair_of(dp[c]);
+                hl[c] = vl[c] * d;
+                hh[c] = vh[c] * d;
+            }
+            LDS unsigned char *vo = B + KF + b * 2048 + g4 * 512 + 16 * r16;
+            *reinterpret_cast<LDS f16x8 *>(vo) = join8(hl[0], hl[1], hl[2], hl[3]);
+            *reinterpret_cast<LDS f16x8 *>(vo + 256) = join8(hh[0], hh[1], hh[2], hh[3]);
+            if constexpr (NS == 2) {
+                f16x2 ll[4], lh[4];
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const f16x2 d = pair_of(dp[c]);
+                    ll[c] = __builtin_elementwise_fma(vl[c], d, -hl[c]);
+                    lh[c] = __builtin_elementwise_fma(vh[c], d, -hh[c]);
+                }
+                *reinterpret_cast<LDS f16x8 *>(vo + VF) = join8(ll[0], ll[1], ll[2], ll[3]);
+                *reinterpret_cast<LDS f16x8 *>(vo + VF + 256) = join8(lh[0], lh[1], lh[2], lh[3]);
+            }
+        }
+    };
+
+    f32x16 O[NB];
+#pragma unroll
+    for (uint32_t b = 0; b < NB; b++) O[b] = f32x16{0.0f};
+    float ref = REF_NONE, lsum = 0.0f;
+    auto compute = [&](int j, uint32_t holes) {
+        const int row0 = c0 + j * (int)TILE;
+        if (row0 >= wmax) return;   // (uniform) no row of the wave sees the tile
+        uint32_t ln = lane;
+        asm volatile("" : "+v"(ln));   // (opaque, as in issue)
+        const uint32_t hf = ln >> 5;
+        const LDS unsigned char *B = F + (j & 1) * BUF;
+        auto fr = [&](uint32_t at) { return *reinterpret_cast<const LDS f16x8 *>(B + at + 16 * ln); };
+        auto q_at = [&](uint32_t m) { return m < QR ? Q[0][m] : ((const LDS f16x8 *)qx)[(w * QL + m - QR) * 64 + ln]; };
+        f32x16 S = {0.0f};
+        if constexpr (!KX) {
+#pragma unroll
+            for (uint32_t m = 0; m < 2 * NB; m++) S = __builtin_amdgcn_mfma_f32_32x32x16_f16(fr(m * 1024), Q[0][m], S, 0, 0, 0);
+        } else {
+#pragma unroll
+            for (uint32_t b = 0; b < NB; b++) {
+                if (b % 2 == 0) sched_fence();
+                const f16x8 k0 = fr(2 * b * 1024), k1 = fr((2 * b + 1) * 1024);
+                f32x16 t = {0.0f};
+                t = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, q_at(2 * b), t, 0, 0, 0);
+                if constexpr (NS == 2) t = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, Q[NS - 1][2 * b], t, 0, 0, 0);
+                t = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, q_at(2 * b + 1), t, 0, 0, 0);
+                if constexpr (NS == 2) t = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, Q[NS - 1][2 * b + 1], t, 0, 0, 0);
+#pragma unroll
+                for (uint32_t i = 0; i < 4; i++) {
+                    const u32x2 d = *reinterpret_cast<const LDS u32x2 *>(B + KF + NS * VF + b * 64 + 16 * i + 8 * hf);
+                    const f16x2 d0 = pair_of(d.x), d1 = pair_of(d.y);
+                    S[4 * i] = fmaf(t[4 * i], (float)d0.x, S[4 * i]);
+                    S[4 * i + 1] = fmaf(t[4 * i + 1], (float)d0.y, S[4 * i + 1]);
+                    S[4 * i + 2] = fmaf(t[4 * i + 2], (float)d1.x, S[4 * i + 2]);
+                    S[4 * i + 3] = fmaf(t[4 * i + 3], (float)d1.y, S[4 * i + 3]);
+                }
+            }
+        }
+        const bool masked = row0 + (int)TILE > wmin || holes != 0;
+        auto sees = [&](uint32_t v) {
+            return row0 + (int)(8 * (v >> 2) + 4 * hf + (v & 3u)) < my_vis && !(holes >> (v >> 3) & 1u);
+        };
+        if (masked) {
+#pragma unroll
+            for (uint32_t v = 0; v < 16; v++) S[v] = sees(v) ? S[v] : -INFINITY;
+        }
+        float mx = S[0];
+#pragma unroll
+        for (uint32_t v = 1; v < 16; v++) mx = fmaxf(mx, S[v]);
+        mx = mx * qs;
+        if (__builtin_amdgcn_ballot_w64(mx > ref + TOP) != 0) {
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            const float nr = fmaxf(ref, mx - FRESH);
+            if (nr != ref) {
+                const float c = __builtin_amdgcn_exp2f(ref - nr);
+                lsum *= c;
+#pragma unroll
+                for (uint32_t b = 0; b < NB; b++)
+#pragma unroll
+                    for (uint32_t v = 0; v < 16; v++) O[b][v] = O[b][v] * c;
+                ref = nr;
+            }
+        }
+        float ps[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (uint32_t v = 0; v < 16; v++) {
+            float p = __builtin_amdgcn_exp2f(fmaf(S[v], qs, -ref));
+            if (masked) p = sees(v) ? p : 0.0f;
+            if constexpr (NP == 2) asm volatile("" : "+v"(p));
+            ps[v & 3u] += p;
+            S[v] = p;
+        }
+        lsum += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+        f16x8 P[NP][2];
+#pragma unroll
+        for (uint32_t s = 0; s < 2; s++)
+#pragma unroll
+            for (uint32_t k = 0; k < 8; k++) {
+                const float p = S[8 * s + ((k & 4) | ((k & 1) << 1) | ((k >> 1) & 1))];   // 0 2 1 3 4 6 5 7
+                P[0][s][k] = (_Float16)p;
+                if constexpr (NP == 2) P[NP - 1][s][k] = (_Float16)(p - (float)P[0][s][k]);
+            }
+#pragma unroll
+        for (uint32_t b = 0; b < NB; b++)
+#pragma unroll
+            for (uint32_t s = 0; s < 2; s++) {
+                const f16x8 v = fr(KF + b * 2048 + s * 1024);
+                O[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, P[0][s], O[b], 0, 0, 0);
+                if constexpr (NP == 2) O[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, P[NP - 1][s], O[b], 0, 0, 0);
+                if constexpr (NS == 2) {
+                    O[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fr(KF + VF + b * 2048 + s * 1024), P[0][s], O[b], 0, 0, 0);
+                }
+            }
+        uint32_t any = 0;
+#pragma unroll
+        for (uint32_t b = 0; b < NB; b++) any |= ((const LDS uint32_t *)odd)[(j & 1) * 8 + b];
+        if (__builtin_expect(__builtin_amdgcn_readfirstlane(any) != 0, 0)) {
+            const int n = my_vis - row0;
+            const uint32_t mine = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
+#pragma unroll
+            for (uint32_t b = 0; b < NB; b++)
+                if (((const LDS uint32_t *)odd)[(j & 1) * 8 + b] & mine) O[b] = O[b] + __builtin_nanf("");
+        }
+    };
+
+    if (n_tile > 0) {
+        In in;
+        issue(0, in);
+        dma_wait();
+        __syncthreads();
+        unpack(0, in);
+        uint32_t holes = in.holes;
+        if (n_tile > 1) issue(1, in);
+        for (int j = 0; j < n_tile; j++) {
+            dma_wait();        // tile j + 1's loads, issued an iteration ago
+            __syncthreads();   // they are in from every wave; tile j is unpacked; tile j - 1 is done with
+            // The two waves of a SIMD take turns: one unpacks (VALU) while the
+            // other's scores run on the matrix core, and so on through a tile
+            const uint32_t h = in.holes;
+            auto fetch = [&] {
+                if (j + 1 < n_tile) unpack(j + 1, in);
+                if (j + 2 < n_tile) issue(j + 2, in);
+            };
+            if (NW == 4 || w < 4) fetch();
+            compute(j, holes);
+            if (NW == 8 && w >= 4) fetch();
+            holes = h;
+        }
+    }
+    // Out through LDS, up to 128 dims of the wave's rows at a time, so that a
+    // row's stores are consecutive: 16-byte unit u of row r in slot u ^ (r % UN)
+    lsum += __shfl_xor(lsum, 32, 64);
+    __syncthreads();   // (every wave is past its last tile: the fragments are free)
+    LDS unsigned char *W = F + w * PASS;
+#pragma unroll
+    for (uint32_t h = 0; h < NB / PB; h++) {
+#pragma unroll
+        for (uint32_t b = 0; b < PB; b++)
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) {
+                const f32x16 &o = O[h * PB + b];
+                *reinterpret_cast<LDS f32x4 *>(W + 16 * (l32 * UN + ((8 * b + 2 * i + hf) ^ (l32 % UN)))) =
+                    f32x4{o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]};
+            }
+#pragma unroll 1
+        for (uint32_t i = lane; i < 32 * UN; i += 64) {
+            const uint32_t r = i / UN, u = i % UN, orow = r0 + 32 * w + r, e = 32 * PB * h + 4 * u;
+            const f32x4 o = *reinterpret_cast<const LDS f32x4 *>(W + 16 * (r * UN + (u ^ (r % UN))));
+            const float l = __shfl(lsum, (int)r, 64), m = __shfl(ref, (int)r, 64);
+            if (orow >= M) continue;
+            if (whole) {
+                store_out(a, wk.tok0 + (int)(orow / a.gqa), g * a.gqa + orow % a.gqa, e, o, l);
+            } else {
+                const size_t rec = (((size_t)gt * NKV + g) * a.n_split + ck) * ROWS + 32 * w + r;
+                *reinterpret_cast<f32x4 *>(a.tpart + rec * HD + e) = o;
+                if (e == 0) a.tml[rec] = make_float2(m, l);
+            }
+        }
+    }
+}
+
+// The chunks of kv4_tile_kernel's rows joined: one wave per (token, q head).
+template <int NW>
+__global__ __launch_bounds__(256) void kv4_join_kernel(Attn a) {
+    constexpr uint32_t ROWS = 32 * NW;
+    const uint32_t u = blockIdx.x * 4u + (threadIdx.x >> 6), lane = threadIdx.x & 63u, HD = a.b.hd;
+    if (u >= a.b.n_tok * a.nq) return;
+    const uint32_t t = u / a.nq, h = u % a.nq;
+    const int seq = seq_of(a.b, t);
+    if (seq < 0) return;
+    const Work wk = find_tile(a, ROWS, (uint32_t)seq, true, false);
+    if (wk.seq < 0) return;
+    const uint32_t i = t - (uint32_t)wk.tok0;
+    if (i >= (uint32_t)wk.n_new || i >= a.max_q) return;
+    const uint32_t g = h / a.gqa, row = i * a.gqa + h % a.gqa, tile = row / ROWS, M = (uint32_t)wk.n_new * a.gqa;
+    const int last = wk.len - wk.n_new + (int)(min(tile * ROWS + ROWS - 1u, M - 1u) / a.gqa);
+    const uint32_t seen = (uint32_t)max(0, min(last + 1, (int)row_cap(a))), per = chunk_rows(seen, a.n_split);
+    if (seen <= per) return;
+    const uint32_t n = (seen + per - 1u) / per;
+    const size_t rec = (((size_t)(wk.first + tile) * a.b.nkv + g) * a.n_split) * ROWS + row % ROWS;
+    float m = REF_NONE, l = 0.0f;
+    for (uint32_t c = 0; c < n; c++) m = fmaxf(m, a.tml[rec + (size_t)c * ROWS].x);
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    const uint32_t e = 4 * lane;
+    for (uint32_t c = 0; c < n; c++) {
+        const float2 ml = a.tml[rec + (size_t)c * ROWS];
+        const f32x4 x = *reinterpret_cast<const f32x4 *>(a.tpart + (rec + (size_t)c * ROWS) * HD + (e < HD ? e : 0u));
+        const float k = __builtin_amdgcn_exp2f(ml.x - m);
+        l = fmaf(ml.y, k, l);
+#pragma unroll
+        for (int j = 0; j < 4; j++) o[j] = fmaf(x[j], k, o[j]);
+    }
+    if (e < HD) store_out(a, t, h, e, o, l);
 }
 
 // ------------------------------------------------------------------ host side
@@ -836,35 +1382,81 @@ int check_attn(const sinter_kv4_batch *b, const sinter_kv4_attn_args *a) {
     return SINTER_OK;
 }
 
-// The launch of a batch: row tiles a sequence and chunk slots.  A slot a
-// sequence, and where there may be rows to split as many more as give every CU
-// two workgroups.
+// Waves of a kv4_tile_kernel workgroup: F32's two parts of q and V fill the
+// registers of one wave a SIMD; else two, and eight waves that unpack together
+// rather than two workgroups of four (500 tokens behind 32,000 rows, 27B heads,
+// bf16: 684 us against 587)
+constexpr uint32_t tile_waves(bool f32) { return f32 ? 4 : 8; }
+
+// The launches of a batch.  kv4_split_kernel: row tiles a sequence and chunk
+// slots, a slot a sequence and, where there may be rows to split, as many more
+// as give every CU some workgroups.  kv4_tile_kernel: row tiles (at most one
+// partly filled one a sequence) and chunks of the cache rows a tile sees.
 struct Plan {
-    uint32_t n_mt, n_slots;
-    bool merge;
-    uint64_t grid;
-    size_t recs;
+    uint32_t n_mt = 0, n_slots = 0, n_tile = 0, n_split = 1;
+    bool split = false, merge = false, join = false;
+    uint64_t grid = 0, tile_grid = 0;
+    size_t recs = 0, tile_recs = 0;
+    size_t bytes(uint32_t hd) const { return (recs + tile_recs) * ((size_t)hd * 4 + 8); }
 };
 Plan make_plan(const sinter_kv4_batch &b, const sinter_kv4_attn_args &a) {
     Plan p;
-    const uint64_t rows = (uint64_t)std::min(a.max_q, b.n_tok) * (a.nq / b.nkv);
-    p.n_mt = (uint32_t)((rows + 15) / 16);
-    p.merge = a.max_kv > CT_MIN * TILE;
-    p.n_slots = b.n_seq;
-    if (p.merge) {
-        const uint64_t per = (uint64_t)b.nkv * p.n_mt;
-        const uint64_t most = (uint64_t)b.n_seq * ((a.max_kv + CT_MIN * TILE - 1) / (CT_MIN * TILE));
-        p.n_slots += (uint32_t)std::min<uint64_t>(std::max<uint64_t>(1, 1024 / per), most);
+    const uint32_t gqa = a.nq / b.nkv;
+    const uint64_t rows = (uint64_t)std::min(a.max_q, b.n_tok) * gqa;
+    // (a sequence that all tokens may belong to, of many rows, is taken whole
+    // by kv4_tile_kernel)
+    p.split = gqa <= SPLIT_ROWS && (rows <= SPLIT_ROWS || b.n_seq > 1);
+    if (p.split) {
+        p.n_mt = (uint32_t)((std::min<uint64_t>(rows, SPLIT_ROWS) + 15) / 16);
+        p.merge = a.max_kv > CT_MIN * TILE;
+        p.n_slots = b.n_seq;
+        if (p.merge) {
+            const uint64_t per = (uint64_t)b.nkv * p.n_mt;
+            const uint64_t most = (uint64_t)b.n_seq * ((a.max_kv + CT_MIN * TILE - 1) / (CT_MIN * TILE));
+            p.n_slots += (uint32_t)std::min<uint64_t>(std::max<uint64_t>(1, 1024 / per), most);
+        }
+        p.grid = (uint64_t)p.n_slots * b.nkv * p.n_mt;
+        p.recs = p.merge ? (size_t)p.grid * 16 : 0;
     }
-    p.grid = (uint64_t)p.n_slots * b.nkv * p.n_mt;
-    p.recs = p.merge ? (size_t)p.grid * 16 : 0;
+    if (!p.split || rows > SPLIT_ROWS) {
+        const uint64_t least = p.split ? SPLIT_ROWS / gqa + 1 : 1;   // tokens of a sequence that comes here
+        const uint32_t tile_rows = 32 * tile_waves(a.type == SINTER_F32);
+        p.n_tile = (uint32_t)((uint64_t)b.n_tok * gqa / tile_rows + std::min<uint64_t>(b.n_seq, b.n_tok / least));
+        const uint64_t wgs = (uint64_t)p.n_tile * b.nkv, room = 256;
+        // Chunks: the fewest cache tiles on the longest way through (rounds
+        // of equal workgroups behind long contexts; the longest tile, or an
+        // even share, of fresh prompts, whose tiles start longest first), a
+        // workgroup's start and end counted as 5 cache tiles, a join as 8
+        const double kv = (a.max_kv + TILE - 1) / TILE, fresh = std::min(1.0, (double)a.max_q / a.max_kv);
+        double best = 1e300;
+        for (uint32_t s = 1; s <= 32 && (s == 1 || a.max_kv / s >= CHUNK_MIN); s++) {
+            const double rounds = std::ceil((double)(wgs * s) / room);
+            const double cost = (fresh < 0.5 ? rounds / s : std::max(1.0 / s, 1.08 * wgs * (1.0 - fresh / 2) / room)) * kv +
+                                5.0 * rounds + (s > 1 ? 8.0 : 0.0);
+            if (cost < best) { best = cost; p.n_split = s; }
+        }
+        p.join = p.n_split > 1;
+        p.tile_grid = wgs * p.n_split;
+        p.tile_recs = p.join ? (size_t)p.tile_grid * tile_rows : 0;
+    }
     return p;
 }
 
 template <int HD>
-void launch_split(const Attn &k, uint32_t grid, hipStream_t s) {
-    if (k.type == SINTER_F32) hipLaunchKernelGGL((kv4_split_kernel<HD, 2>), dim3(grid), dim3(256), 0, s, k);
-    else hipLaunchKernelGGL((kv4_split_kernel<HD, 1>), dim3(grid), dim3(256), 0, s, k);
+void launch_attn(const Attn &k, const Plan &p, hipStream_t s) {
+    const bool f32 = k.type == SINTER_F32;
+    if (p.tile_grid) {
+        auto tile = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3((uint32_t)p.tile_grid), dim3(64 * tile_waves(f32)), 0, s, k);
+        };
+        if (f32) tile(kv4_tile_kernel<HD, SINTER_F32, tile_waves(true)>);
+        else if (k.type == SINTER_F16) tile(kv4_tile_kernel<HD, SINTER_F16, tile_waves(false)>);
+        else tile(kv4_tile_kernel<HD, SINTER_BF16, tile_waves(false)>);
+    }
+    if (p.grid) {
+        if (f32) hipLaunchKernelGGL((kv4_split_kernel<HD, 2>), dim3((uint32_t)p.grid), dim3(256), 0, s, k);
+        else hipLaunchKernelGGL((kv4_split_kernel<HD, 1>), dim3((uint32_t)p.grid), dim3(256), 0, s, k);
+    }
 }
 
 }  // namespace
@@ -960,7 +1552,7 @@ int sinter_kv4_read(const sinter_kv4_batch *b, const sinter_heads *k, const sint
 
 size_t sinter_kv4_attn_ws_bytes(const sinter_kv4_batch *b, const sinter_kv4_attn_args *a) {
     if (check_attn(b, a) != SINTER_OK || b->n_seq == 0 || b->n_tok == 0) return 0;
-    return make_plan(*b, *a).recs * ((size_t)b->hd * 4 + 8);
+    return make_plan(*b, *a).bytes(b->hd);
 }
 
 int sinter_kv4_attn(const sinter_kv4_batch *b, const sinter_kv4_attn_args *a, void *stream) {
@@ -972,26 +1564,38 @@ int sinter_kv4_attn(const sinter_kv4_batch *b, const sinter_kv4_attn_args *a, vo
         (a->gate.p && (why = check_heads(a->gate, b->n_tok, a->nq, b->hd, (int)a->type))))
         return set_error(SINTER_ERR_ARG, "kv4_attn: %s", why);
     const Plan p = make_plan(*b, *a);
-    const size_t need = p.recs * ((size_t)b->hd * 4 + 8);
+    const size_t need = p.bytes(b->hd);
     if (need && (!a->ws || (uintptr_t)a->ws % 16u || a->ws_bytes < need))
         return set_error(SINTER_ERR_ARG, "kv4_attn: workspace of %zu bytes, 16-byte aligned (sinter_kv4_attn_ws_bytes)", need);
-    if (p.grid > (uint64_t)INT32_MAX || (uint64_t)b->n_tok * a->nq > (uint64_t)INT32_MAX)
+    if (p.grid > (uint64_t)INT32_MAX || p.tile_grid > (uint64_t)INT32_MAX || (uint64_t)b->n_tok * a->nq > (uint64_t)INT32_MAX ||
+        (p.merge && (uint64_t)b->n_seq * b->nkv * SPLIT_ROWS > (uint64_t)INT32_MAX))
         return set_error(SINTER_ERR_ARG, "kv4_attn: batch too large");
     Attn k;
     k.b = *b;
     k.q = a->q; k.gate = a->gate; k.out = a->out;
     k.part = static_cast<float *>(a->ws);
-    k.ml = reinterpret_cast<float2 *>(k.part + p.recs * b->hd);
+    k.tpart = k.part + p.recs * b->hd;
+    k.ml = reinterpret_cast<float2 *>(k.tpart + p.tile_recs * b->hd);
+    k.tml = k.ml + p.recs;
     k.nq = a->nq; k.gqa = a->nq / b->nkv; k.max_q = a->max_q; k.max_kv = a->max_kv;
     k.n_slots = p.n_slots; k.n_mt = p.n_mt; k.type = a->type;
+    k.n_tile = p.n_tile; k.n_split = p.n_split; k.report = !p.split; k.split_rows = p.split ? SPLIT_ROWS : 0;
     k.page_shift = (uint32_t)__builtin_ctz(b->page_rows);
     k.qscale = a->scale * 1.44269504088896341f;
     const hipStream_t s = (hipStream_t)stream;
-    if (b->hd == 256) launch_split<256>(k, (uint32_t)p.grid, s);
-    else if (b->hd == 128) launch_split<128>(k, (uint32_t)p.grid, s);
-    else launch_split<64>(k, (uint32_t)p.grid, s);
+    if (b->hd == 256) launch_attn<256>(k, p, s);
+    else if (b->hd == 128) launch_attn<128>(k, p, s);
+    else launch_attn<64>(k, p, s);
     if (!hip_ok(hipGetLastError(), "kv4_attn: launch")) return SINTER_ERR_HIP;
-    if (p.merge) hipLaunchKernelGGL(kv4_merge_kernel, dim3(b->n_tok * a->nq), dim3(256), 0, s, k);
+    const uint32_t out_rows = b->n_tok * a->nq;
+    if (p.join) {
+        if (a->type == SINTER_F32) hipLaunchKernelGGL((kv4_join_kernel<tile_waves(true)>), dim3((out_rows + 3) / 4), dim3(256), 0, s, k);
+        else hipLaunchKernelGGL((kv4_join_kernel<tile_waves(false)>), dim3((out_rows + 3) / 4), dim3(256), 0, s, k);
+    }
+    if (p.merge) {
+        const uint32_t rows = std::min(std::min(a->max_q, b->n_tok) * k.gqa, SPLIT_ROWS / k.gqa * k.gqa);
+        hipLaunchKernelGGL(kv4_merge_kernel, dim3(b->n_seq * b->nkv * rows), dim3(256), 0, s, k, rows);
+    }
     return hip_ok(hipGetLastError(), "kv4_attn: merge launch") ? SINTER_OK : SINTER_ERR_HIP;
 }
 

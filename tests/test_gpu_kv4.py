@@ -20,7 +20,9 @@ over rows add at most 2^-18 (tiles, waves and chunks of at most 64 each on top
 of the 32 rows of a tile), and a term of a row of n is off by at least f16's
 smallest step, 2^-25 at a largest weight of at least 2^4 / (scale bound): n 2^-26
 of the largest |v|.  All of it in sum w |v|, then the gate's 8 u and the
-type's half step.
+type's half step.  Sequences of more than 32 (token, head) rows run on tiles
+unpacked to f16: V's scale * code is rounded (2^-11 of sum w |v|; F32 keeps the
+rest in a second part), and for BF16 K's too, 2^-11 of sum |q k| in a score.
 """
 import ctypes as C
 
@@ -277,9 +279,13 @@ def check_attn(b, nq, t, q, got, gate, scale, untouched=3.0, only=None):
             k, v = kv[s][0][h // gqa, :max(0, p + 1)], kv[s][1][h // gqa, :max(0, p + 1)]
             with np.errstate(all="ignore"):
                 want, mag, qk = ref.attention(q[j, h], k, v, scale)
-            n = len(k)
+            n, many = len(k), int(b.tok_start[s + 1] - b.tok_start[s]) * gqa > 32
             score = 40 * U * qk + (2.0 ** -22 * qk if t == F32 else 0) + 8 * U * qk + 8 * U
+            if many and t == BF16:
+                score += 2.0 ** -11 * qk
             rel = 2 * score + (2.0 ** -22 if t == F32 else 2.0 ** -11) + 2.0 ** -18
+            if many and t != F32:
+                rel += 2.0 ** -11
             err = rel * mag + n * 2.0 ** -26 * (np.abs(v).max() if n else 0)
             if gate is not None:
                 sg = 1.0 / (1.0 + np.exp(-gate[j, h]))
@@ -346,15 +352,16 @@ def test_attention_many_sequences(sn, torch_gpu, n_seq):
     check_attn(b, 2, BF16, q, got, g, 64 ** -0.5)
 
 
-@pytest.mark.parametrize("t", [F32, F16])
-def test_attention_magnitudes(sn, torch_gpu, t):
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+@pytest.mark.parametrize("toks", [2, 30])
+def test_attention_magnitudes(sn, torch_gpu, t, toks):
     """Tiny and huge values, scales that grow along the sequence and differ by
     block, scores that keep growing: the weights' reference moves."""
     torch = torch_gpu
     hd, n = 128, 700
-    b = Batch(sn, torch, [2], [n], 64, 1, hd, seed=4)
+    b = Batch(sn, torch, [toks], [n], 64, 1, hd, seed=4)
     rng = np.random.default_rng(8)
-    q = rng.standard_normal((2, 4, hd)).astype(np.float32)
+    q = rng.standard_normal((toks, 4, hd)).astype(np.float32)
     q[0, 1] *= 1e-3
     if t == F32:
         q[1, 2] *= 1e20
@@ -374,9 +381,12 @@ def test_attention_magnitudes(sn, torch_gpu, t):
 
 
 @pytest.mark.parametrize("nan", [0x7e00, 0x7c00])
-def test_attention_rows_not_seen_stay_out(sn, torch_gpu, nan):
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+@pytest.mark.parametrize("nq", [6, 14])
+def test_attention_rows_not_seen_stay_out(sn, torch_gpu, nan, t, nq):
     """A later token's row that is not finite reaches only the tokens that see it."""
     torch = torch_gpu
+    half = nq // 2
     b = Batch(sn, torch, [9], [50], 16, 2, 64, seed=3)
     b.fill_rows(5)
     for cache in (b.kc, b.vc):
@@ -384,23 +394,22 @@ def test_attention_rows_not_seen_stay_out(sn, torch_gpu, nan):
             _, sc = ref.head_view(cache, b.pages[0, r // 16], 1, 16, 2, 64)
             sc.view(np.uint16)[r % 16, 1] = nan
     b.up()
-    q = np.random.default_rng(1).standard_normal((9, 6, 64)).astype(np.float32)
-    (_, qv), (_, ov) = strided(torch, q, F32), strided(torch, np.zeros_like(q), F32)
-    a, ws = attn_args(sn, torch, b, 6, F32, qv, ov)
+    q = np.random.default_rng(1).standard_normal((9, nq, 64)).astype(np.float32)
+    (_, qv), (_, ov) = strided(torch, q, t), strided(torch, np.zeros_like(q), t)
+    a, ws = attn_args(sn, torch, b, nq, t, qv, ov)
     ok(sn, sn.lib().sinter_kv4_attn(C.byref(b.rec()), C.byref(a), stream(torch)), torch)
-    got = ov.cpu().numpy()
-    assert np.isfinite(got[:4]).all() and np.isfinite(got[:, :3]).all()
-    assert not np.isfinite(got[4:, 3:]).all(-1).any()
-    bb = Batch(sn, torch, [4], [45], 16, 2, 64, seed=3)   # the tokens before row 45 on their own
-    bb.kc, bb.vc, bb.pages, bb.n_pages, bb.max_pages = b.kc, b.vc, b.pages, b.n_pages, b.max_pages
-    check_attn(bb, 6, F32, q[:4].astype(np.float64), got[:4], None, 64 ** -0.5)
+    got = ov.float().cpu().numpy()
+    assert np.isfinite(got[:4]).all() and np.isfinite(got[:, :half]).all()
+    assert not np.isfinite(got[4:, half:]).all(-1).any()
+    check_attn(b, nq, t, qv.double().cpu().numpy(), got, None, 64 ** -0.5, only=(0, 1, 2, 3))
 
 
-def test_attention_nonfinite_query_stays_alone(sn, torch_gpu):
+@pytest.mark.parametrize("n", [3, 20])
+def test_attention_nonfinite_query_stays_alone(sn, torch_gpu, n):
     torch = torch_gpu
-    b = Batch(sn, torch, [3], [70], 16, 1, 64, seed=3)
+    b = Batch(sn, torch, [n], [70], 16, 1, 64, seed=3)
     b.fill_rows(5)
-    q = np.random.default_rng(1).standard_normal((3, 2, 64)).astype(np.float32)
+    q = np.random.default_rng(1).standard_normal((n, 2, 64)).astype(np.float32)
     q[1, 0, 7] = np.nan
     q[2, 1, 9] = np.inf
     (_, qv), (_, ov) = strided(torch, q, F32), strided(torch, np.zeros_like(q), F32)
@@ -408,7 +417,7 @@ def test_attention_nonfinite_query_stays_alone(sn, torch_gpu):
     ok(sn, sn.lib().sinter_kv4_attn(C.byref(b.rec()), C.byref(a), stream(torch)), torch)
     got = ov.cpu().numpy()
     assert np.isnan(got[1, 0]).all()
-    fine = np.ones((3, 2), bool)
+    fine = np.ones((n, 2), bool)
     fine[1, 0] = fine[2, 1] = False
     assert np.isfinite(got[fine]).all()
 
