@@ -405,14 +405,31 @@ __device__ __forceinline__ void lds_dma16v(uint64_t addr, uint32_t lds_base) {
 // Eight codes as f16 integers -8..7: the low (or high) four bits of two words'
 // bytes, in the order bytes 0 2 1 3 of `x`, then of `y`.  0x6400 | q is 1024 +
 // q; in the high bits 1024 + 16 q, brought down by an exact product and sum.
+// (one v_and_or_b32, its constants in registers: the compiler's choice is an
+// and and an or with a literal each)
+__device__ __forceinline__ f16x2 and_or(uint32_t w, uint32_t mask, uint32_t bits) {
+    uint32_t r;
+    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(w), "s"(mask), "v"(bits));
+    return pair_of(r);
+}
 __device__ __forceinline__ f16x2 code_pair_lo(uint32_t w) {
-    const f16x2 v = __builtin_bit_cast(f16x2, (w & 0x000f000fu) | 0x64006400u);
-    return v + f16x2{(_Float16)-1032.0f, (_Float16)-1032.0f};
+    return and_or(w, 0x000f000fu, 0x64006400u) + f16x2{(_Float16)-1032.0f, (_Float16)-1032.0f};
 }
 __device__ __forceinline__ f16x2 code_pair_hi(uint32_t w) {
-    const f16x2 v = __builtin_bit_cast(f16x2, (w & 0x00f000f0u) | 0x64006400u);
-    return __builtin_elementwise_fma(v, f16x2{(_Float16)0.0625f, (_Float16)0.0625f},
+    return __builtin_elementwise_fma(and_or(w, 0x00f000f0u, 0x64006400u), f16x2{(_Float16)0.0625f, (_Float16)0.0625f},
                                      f16x2{(_Float16)-72.0f, (_Float16)-72.0f});
+}
+// A branch around rare work, not selects beside the common: the compiler moves
+// nothing past it
+__device__ __forceinline__ void keep_branch() { asm volatile(""); }
+// p in two f16 parts
+__device__ __forceinline__ void split2(float p0, float p1, f16x2 &hi, f16x2 &lo) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    // (opaque: a product rounded to fp16 straight in one place and by way of
+    // fp32 in the other, the parts would not add up)
+    asm("" : "+v"(p0), "+v"(p1));
+    hi = __builtin_convertvector((f32x2{p0, p1}), f16x2);
+    lo = __builtin_convertvector((f32x2{fmaf(p0, 1.0f, -(float)hi.x), fmaf(p1, 1.0f, -(float)hi.y)}), f16x2);
 }
 __device__ __forceinline__ f16x8 join8(f16x2 a, f16x2 b, f16x2 c, f16x2 d) {
     return f16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
@@ -640,25 +657,23 @@ __global__ __launch_bounds__(256, 2) void kv4_split_kernel(Attn a) {
             }
         }
         // a tile with rows that some row here does not see
-        const bool masked = row0 + (int)TILE > min(end, pmin + 1) || hole != 0;
+        const bool masked = __builtin_amdgcn_readfirstlane(row0 + (int)TILE > min(end, pmin + 1) || hole != 0 ? 1 : 0) != 0;
         float p[8];
-        bool ok[8];
 #pragma unroll
-        for (uint32_t k = 0; k < 8; k++) {
-            p[k] = s[k >> 2][k & 3] * qs;
-            ok[k] = true;
-        }
+        for (uint32_t k = 0; k < 8; k++) p[k] = s[k >> 2][k & 3];
         if (masked) {
+            keep_branch();
 #pragma unroll
             for (uint32_t k = 0; k < 8; k++) {
-                ok[k] = row0 + (int)(16 * (k >> 2) + 4 * g4 + (k & 3)) < my_vis && !(hole >> (k >> 2) & 1u);
-                p[k] = ok[k] ? p[k] : -INFINITY;
+                const bool ok = row0 + (int)(16 * (k >> 2) + 4 * g4 + (k & 3)) < my_vis && !(hole >> (k >> 2) & 1u);
+                p[k] = ok ? p[k] : -INFINITY;
                 // (a masked row's scale may be anything: 0 keeps it out)
 #pragma unroll
-                for (uint32_t b = 0; b < NB / 2; b++) dv[k][b] = ok[k] ? dv[k][b] : 0u;
+                for (uint32_t b = 0; b < NB / 2; b++) dv[k][b] = ok ? dv[k][b] : 0u;
             }
         }
         float mx = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
+        mx = mx * qs;
         if (__builtin_amdgcn_ballot_w64(mx > lim || dm > dtop) != 0) {
             dm = wave_max_f32(dm);
             if (dm > dtop) {   // (uniform) to twice the largest, a power of two
@@ -679,8 +694,7 @@ __global__ __launch_bounds__(256, 2) void kv4_split_kernel(Attn a) {
         }
 #pragma unroll
         for (uint32_t k = 0; k < 8; k++) {
-            p[k] = __builtin_amdgcn_exp2f(p[k] - ref);
-            if (masked) p[k] = ok[k] ? p[k] : 0.0f;
+            p[k] = __builtin_amdgcn_exp2f(fmaf(p[k], qs, -ref));   // (0 where masked)
             lsum += p[k];
         }
         // V^T: lane i of a group of 16 reads half i % 2 of row key(i / 2) and
@@ -688,7 +702,7 @@ __global__ __launch_bounds__(256, 2) void kv4_split_kernel(Attn a) {
         const uint32_t kr = (r16 >> 1), vr = 16 * (kr >> 2) + 4 * g4 + (kr & 3);
 #pragma unroll
         for (uint32_t b = 0; b < NB; b++) {
-            if (b % 2 == 0) sched_fence();
+            if (NS == 2 || b % 2 == 0) sched_fence();
             const i32x2 x = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
                 (LDS i32x2 *)(vt + vr * HB + 16 * (b ^ swz(vr)) + 8 * (r16 & 1u)));
             const uint32_t x0 = (uint32_t)x.x, x1 = (uint32_t)x.y;
@@ -696,20 +710,18 @@ __global__ __launch_bounds__(256, 2) void kv4_split_kernel(Attn a) {
             const f16x8 Ah = join8(code_pair_hi(x0), code_pair_hi(x0 >> 8), code_pair_hi(x1), code_pair_hi(x1 >> 8));
             f16x8 P, Pl;
 #pragma unroll
-            for (uint32_t k = 0; k < 8; k++) {
-                const uint32_t key = (k & 4) | ((k & 1) << 1) | ((k >> 1) & 1);   // 0 2 1 3 4 6 5 7
-                const f16x2 dd = pair_of(dv[key][b / 2]);
-                const float dk = (float)(b & 1 ? dd.y : dd.x);
+            for (uint32_t k = 0; k < 8; k += 2) {   // keys 0 2, 1 3, 4 6, 5 7
+                const uint32_t k0 = (k & 4) | ((k >> 1) & 1), k1 = k0 + 2;
+                const f16x2 d0 = pair_of(dv[k0][b / 2]), d1 = pair_of(dv[k1][b / 2]);
+                const float s0 = (float)(b & 1 ? d0.y : d0.x), s1 = (float)(b & 1 ? d1.y : d1.x);
                 if constexpr (NS == 1) {
-                    P[k] = (_Float16)fmaf(p[key], dk, 0.0f);
+                    P[k] = (_Float16)fmaf(p[k0], s0, 0.0f);
+                    P[k + 1] = (_Float16)fmaf(p[k1], s1, 0.0f);
                 } else {
-                    // (opaque: rounded to f16 straight from the product in one
-                    // place and from the fp32 product in the other, the parts
-                    // would not add up)
-                    float x = p[key] * dk;
-                    asm volatile("" : "+v"(x));
-                    P[k] = (_Float16)x;
-                    Pl[k] = (_Float16)(x - (float)P[k]);
+                    f16x2 hi, lo;
+                    split2(fmaf(p[k0], s0, 0.0f), fmaf(p[k1], s1, 0.0f), hi, lo);
+                    P[k] = hi.x; P[k + 1] = hi.y;
+                    Pl[k] = lo.x; Pl[k + 1] = lo.y;
                 }
             }
             O[2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(Al, P, O[2 * b], 0, 0, 0);
@@ -898,19 +910,20 @@ __device__ __forceinline__ uint32_t chunk_rows(uint32_t seen, uint32_t n_split) 
 template <int HD, int T, int NW>
 __global__ __launch_bounds__(64 * NW, T == SINTER_F32 ? 1 : 2) void kv4_tile_kernel(Attn a) {
     constexpr uint32_t NS = T == SINTER_F32 ? 2 : 1, NP = T == SINTER_BF16 ? 1 : 2;   // f16 parts of q (and V), of the weights
-    constexpr bool KX = T != SINTER_BF16;
+    constexpr bool KX = T == SINTER_F16;   // exact codes of K in the fragments
     constexpr uint32_t NB = HD / 32, HB = HD / 2, SB = HD / 16, NCH = HB / 16, KC = TILE * HB, ROWS = 32 * NW;
     constexpr uint32_t SH = HD == 256 ? 1 : HD == 128 ? 2 : 3, BPW = NB > NW ? NB / NW : 1, ACT = NB / BPW;
-    constexpr uint32_t KF = NB * 2048, VF = NB * 2048, KS = KX ? NB * 64 : 0, BUF = KF + NS * VF + KS;
+    constexpr uint32_t KF = NS * NB * 2048, VF = NB * 2048, KS = KX ? NB * 64 : 0, BUF = KF + NS * VF + KS;
     // (the output's passes: blocks of 32 dims a pass, 16-byte units a row, bytes a wave)
     constexpr uint32_t FIT = 2 * BUF / (NW * 4096), PB = FIT >= 4 && NB >= 4 ? 4 : FIT >= 2 ? 2 : 1, UN = PB * 8, PASS = PB * 4096;
     __shared__ __attribute__((aligned(16))) unsigned char frag[2 * BUF > NW * PASS ? 2 * BUF : NW * PASS];
     __shared__ __attribute__((aligned(16))) unsigned char raw[2 * KC];
     __shared__ __attribute__((aligned(16))) _Float16 vsc[NB][32];
     __shared__ __attribute__((aligned(16))) uint32_t odd[2][8];
-    // (F16 rows of 256: a block's sums beside the scores leave no registers
-    // for all of q, the last QL slices are read from LDS)
-    constexpr uint32_t QL = HD == 256 && KX && NS == 1 ? 4 : 0, QR = 2 * NB - QL;
+    // (Heads of 256: the sums and q leave too few registers for fragments read
+    // ahead, and for F16 a block's own sums: the last QL slices of q are read
+    // from LDS)
+    constexpr uint32_t QL = HD != 256 || NS == 2 ? 0 : KX ? 4 : 2, QR = 2 * NB - QL;
     __shared__ __attribute__((aligned(16))) f16x8 qx[QL ? NW * QL * 64 : 1];
     const uint32_t lane = threadIdx.x & 63u, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t l32 = lane & 31u, hf = lane >> 5, NKV = a.b.nkv;
@@ -1092,10 +1105,21 @@ __global__ __launch_bounds__(64 * NW, T == SINTER_F32 ? 1 : 2) void kv4_tile_ker
             f16x2 kh[4] = {code_pair_hi(in.k[i].x), code_pair_hi(in.k[i].x >> 8), code_pair_hi(in.k[i].y), code_pair_hi(in.k[i].y >> 8)};
             if constexpr (!KX) {
                 const _Float16 d = __builtin_bit_cast(_Float16, (uint16_t)(real ? in.sc[i] : 0u));
+                const f16x2 dd = {d, d};
+                f16x2 rl[4], rh[4];   // (F32: what the rounded products leave)
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
-                    kl[c] = kl[c] * f16x2{d, d};
-                    kh[c] = kh[c] * f16x2{d, d};
+                    const f16x2 l = kl[c] * dd, h = kh[c] * dd;
+                    if constexpr (NS == 2) {
+                        rl[c] = __builtin_elementwise_fma(kl[c], dd, -l);
+                        rh[c] = __builtin_elementwise_fma(kh[c], dd, -h);
+                    }
+                    kl[c] = l;
+                    kh[c] = h;
+                }
+                if constexpr (NS == 2) {
+                    *reinterpret_cast<LDS f16x8 *>(B + KF / 2 + (2 * b) * 1024 + 16 * ln) = join8(rl[0], rl[1], rl[2], rl[3]);
+                    *reinterpret_cast<LDS f16x8 *>(B + KF / 2 + (2 * b + 1) * 1024 + 16 * ln) = join8(rh[0], rh[1], rh[2], rh[3]);
                 }
             } else if (hf == 0) {
                 ((LDS u16a *)(B + KF + NS * VF))[b * 32 + l32] = (uint16_t)(real ? in.sc[i] : 0u);
@@ -1137,6 +1161,15 @@ __global__ __launch_bounds__(64 * NW, T == SINTER_F32 ? 1 : 2) void kv4_tile_ker
 #pragma unroll
     for (uint32_t b = 0; b < NB; b++) O[b] = f32x16{0.0f};
     float ref = REF_NONE, lsum = 0.0f;
+    // (F32's sums stay in the accumulation half of the registers: left to the
+    // compiler they are copied out and back around the rare paths)
+    auto pin = [&] {
+        if constexpr (T == SINTER_F32) {
+#pragma unroll
+            for (uint32_t b = 0; b < NB; b++) asm volatile("" : "+a"(O[b]));
+        }
+    };
+    pin();
     auto compute = [&](int j, uint32_t holes) {
         const int row0 = c0 + j * (int)TILE;
         if (row0 >= wmax) return;   // (uniform) no row of the wave sees the tile
@@ -1148,8 +1181,26 @@ __global__ __launch_bounds__(64 * NW, T == SINTER_F32 ? 1 : 2) void kv4_tile_ker
         auto q_at = [&](uint32_t m) { return m < QR ? Q[0][m] : ((const LDS f16x8 *)qx)[(w * QL + m - QR) * 64 + ln]; };
         f32x16 S = {0.0f};
         if constexpr (!KX) {
+            f16x8 kf[3], kr[3];
 #pragma unroll
-            for (uint32_t m = 0; m < 2 * NB; m++) S = __builtin_amdgcn_mfma_f32_32x32x16_f16(fr(m * 1024), Q[0][m], S, 0, 0, 0);
+            for (uint32_t m = 0; m < 2; m++) {
+                kf[m] = fr(m * 1024);
+                if constexpr (NS == 2) kr[m] = fr(KF / 2 + m * 1024);
+            }
+#pragma unroll
+            for (uint32_t m = 0; m < 2 * NB; m++) {
+                const f16x8 k = kf[m % 3], r = kr[m % 3];
+                if (m + 2 < 2 * NB) {   // (two slices ahead of the matrix core)
+                    kf[(m + 2) % 3] = fr((m + 2) * 1024);
+                    if constexpr (NS == 2) kr[(m + 2) % 3] = fr(KF / 2 + (m + 2) * 1024);
+                }
+                S = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q_at(m), S, 0, 0, 0);
+                if constexpr (NS == 2) {
+                    S = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, Q[NS - 1][m], S, 0, 0, 0);
+                    S = __builtin_amdgcn_mfma_f32_32x32x16_f16(r, Q[0][m], S, 0, 0, 0);
+                }
+                sched_fence();
+            }
         } else {
 #pragma unroll
             for (uint32_t b = 0; b < NB; b++) {
@@ -1157,9 +1208,7 @@ __global__ __launch_bounds__(64 * NW, T == SINTER_F32 ? 1 : 2) void kv4_tile_ker
                 const f16x8 k0 = fr(2 * b * 1024), k1 = fr((2 * b + 1) * 1024);
                 f32x16 t = {0.0f};
                 t = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, q_at(2 * b), t, 0, 0, 0);
-                if constexpr (NS == 2) t = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, Q[NS - 1][2 * b], t, 0, 0, 0);
                 t = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, q_at(2 * b + 1), t, 0, 0, 0);
-                if constexpr (NS == 2) t = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, Q[NS - 1][2 * b + 1], t, 0, 0, 0);
 #pragma unroll
                 for (uint32_t i = 0; i < 4; i++) {
                     const u32x2 d = *reinterpret_cast<const LDS u32x2 *>(B + KF + NS * VF + b * 64 + 16 * i + 8 * hf);
@@ -1171,11 +1220,12 @@ __global__ __launch_bounds__(64 * NW, T == SINTER_F32 ? 1 : 2) void kv4_tile_ker
                 }
             }
         }
-        const bool masked = row0 + (int)TILE > wmin || holes != 0;
+        const bool masked = __builtin_amdgcn_readfirstlane(row0 + (int)TILE > wmin || holes != 0 ? 1 : 0) != 0;
         auto sees = [&](uint32_t v) {
             return row0 + (int)(8 * (v >> 2) + 4 * hf + (v & 3u)) < my_vis && !(holes >> (v >> 3) & 1u);
         };
         if (masked) {
+            keep_branch();
 #pragma unroll
             for (uint32_t v = 0; v < 16; v++) S[v] = sees(v) ? S[v] : -INFINITY;
         }
@@ -1195,37 +1245,51 @@ __global__ __launch_bounds__(64 * NW, T == SINTER_F32 ? 1 : 2) void kv4_tile_ker
                     for (uint32_t v = 0; v < 16; v++) O[b][v] = O[b][v] * c;
                 ref = nr;
             }
+            pin();
         }
         float ps[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (uint32_t v = 0; v < 16; v++) {
-            float p = __builtin_amdgcn_exp2f(fmaf(S[v], qs, -ref));
-            if (masked) p = sees(v) ? p : 0.0f;
-            if constexpr (NP == 2) asm volatile("" : "+v"(p));
-            ps[v & 3u] += p;
-            S[v] = p;
+            S[v] = __builtin_amdgcn_exp2f(fmaf(S[v], qs, -ref));   // (0 where masked)
+            ps[v & 3u] += S[v];
         }
         lsum += (ps[0] + ps[1]) + (ps[2] + ps[3]);
         f16x8 P[NP][2];
 #pragma unroll
         for (uint32_t s = 0; s < 2; s++)
 #pragma unroll
-            for (uint32_t k = 0; k < 8; k++) {
-                const float p = S[8 * s + ((k & 4) | ((k & 1) << 1) | ((k >> 1) & 1))];   // 0 2 1 3 4 6 5 7
-                P[0][s][k] = (_Float16)p;
-                if constexpr (NP == 2) P[NP - 1][s][k] = (_Float16)(p - (float)P[0][s][k]);
-            }
-#pragma unroll
-        for (uint32_t b = 0; b < NB; b++)
-#pragma unroll
-            for (uint32_t s = 0; s < 2; s++) {
-                const f16x8 v = fr(KF + b * 2048 + s * 1024);
-                O[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, P[0][s], O[b], 0, 0, 0);
-                if constexpr (NP == 2) O[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, P[NP - 1][s], O[b], 0, 0, 0);
-                if constexpr (NS == 2) {
-                    O[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fr(KF + VF + b * 2048 + s * 1024), P[0][s], O[b], 0, 0, 0);
+            for (uint32_t k = 0; k < 8; k += 2) {   // keys 0 2, 1 3, 4 6, 5 7
+                const float p0 = S[8 * s + (k & 4) + ((k >> 1) & 1)], p1 = S[8 * s + (k & 4) + ((k >> 1) & 1) + 2];
+                if constexpr (NP == 2) {
+                    f16x2 hi, lo;
+                    split2(p0, p1, hi, lo);
+                    P[0][s][k] = hi.x; P[0][s][k + 1] = hi.y;
+                    P[NP - 1][s][k] = lo.x; P[NP - 1][s][k + 1] = lo.y;
+                } else {
+                    P[0][s][k] = (_Float16)p0;
+                    P[0][s][k + 1] = (_Float16)p1;
                 }
             }
+        f16x8 vf[3], vr[3];
+#pragma unroll
+        for (uint32_t m = 0; m < 2; m++) {
+            vf[m] = fr(KF + m * 1024);
+            if constexpr (NS == 2) vr[m] = fr(KF + VF + m * 1024);
+        }
+#pragma unroll
+        for (uint32_t m = 0; m < 2 * NB; m++) {   // block m / 2, keys 16 (m % 2) ..
+            const uint32_t b = m / 2, s = m & 1u;
+            const f16x8 v = vf[m % 3], r = vr[m % 3];
+            if (m + 2 < 2 * NB) {
+                vf[(m + 2) % 3] = fr(KF + (m + 2) * 1024);
+                if constexpr (NS == 2) vr[(m + 2) % 3] = fr(KF + VF + (m + 2) * 1024);
+            }
+            O[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, P[0][s], O[b], 0, 0, 0);
+            if constexpr (NP == 2) O[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, P[NP - 1][s], O[b], 0, 0, 0);
+            if constexpr (NS == 2) O[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(r, P[0][s], O[b], 0, 0, 0);
+            sched_fence();
+        }
+        pin();
         uint32_t any = 0;
 #pragma unroll
         for (uint32_t b = 0; b < NB; b++) any |= ((const LDS uint32_t *)odd)[(j & 1) * 8 + b];
@@ -1235,6 +1299,7 @@ __global__ __launch_bounds__(64 * NW, T == SINTER_F32 ? 1 : 2) void kv4_tile_ker
 #pragma unroll
             for (uint32_t b = 0; b < NB; b++)
                 if (((const LDS uint32_t *)odd)[(j & 1) * 8 + b] & mine) O[b] = O[b] + __builtin_nanf("");
+            pin();
         }
     };
 
