@@ -17,6 +17,7 @@
 // LDS-DMA with nothing read twice.  Element = scale * (code - 8).
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "dev_common.h"
 #include "internal.h"
@@ -263,15 +264,16 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Rows a) {
 
 // ------------------------------------------------------------------ attention
 
-// Chunks of a sequence's rows that one workgroup takes, in 32-row tiles:
-// at least CT_MIN (below it a workgroup's start costs more than its rows)
-constexpr uint32_t TILE = 32, CT_MIN = 16;
+constexpr uint32_t TILE = 32;   // cache rows a tile
+// Tiles a slot of kv4_split_kernel takes at least (two a wave), and the tiles
+// up to which a sequence is not divided (its join would cost more)
+constexpr uint32_t CT_MIN = 8, WHOLE = 16;
 
 struct Attn {
     sinter_kv4_batch b;
     sinter_heads q, gate, out;
-    float *part;     // [slot][kv head][row tile][16][hd] unnormalised sums
-    float2 *ml;      // [slot][kv head][row tile][16] reference and weight sum
+    float *part;     // [slot][2][kv head][row tile][16][hd] unnormalised sums
+    float2 *ml;      // [slot][2][kv head][row tile][16] reference and weight sum
     float *tpart;    // kv4_tile_kernel's: [tile][kv head][chunk][tile rows][hd]
     float2 *tml;
     uint32_t nq, gqa, max_q, max_kv, n_slots, n_mt, type, page_shift;
@@ -288,7 +290,7 @@ constexpr uint32_t SPLIT_ROWS = 32;
 
 struct Work {
     int seq, len, tok0, n_new;   // the sequence: rows, first token, tokens (seq < 0: none)
-    uint32_t item, first;        // the item of it, the number of its item 0
+    uint32_t item, first, count; // the item of it, the number of its item 0, its items
 };
 
 // the most rows of a sequence that the launch and the page table have room for
@@ -312,68 +314,83 @@ __device__ __forceinline__ void load_seq(const Attn &a, uint32_t base, bool repo
     len = max(0, len);
 }
 
+// inclusive sum over the lanes (every lane active)
+__device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v) {
+    auto step = [&](auto ctrl, auto rows) {
+        v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+    };
+    using std::integral_constant;
+    const integral_constant<int, 0xf> all;
+    step(integral_constant<int, 0x111>{}, all);   // row_shr 1, 2, 4, 8
+    step(integral_constant<int, 0x112>{}, all);
+    step(integral_constant<int, 0x114>{}, all);
+    step(integral_constant<int, 0x118>{}, all);
+    step(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});   // row_bcast 15 into rows 1 and 3
+    step(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});   // row_bcast 31 into rows 2 and 3
+    return v;
+}
+
 // The sequences' items, count(len, n) each, numbered one sequence after the
 // other: item `id`'s sequence, or (by_seq) sequence `id` with its item 0.
 template <class Count>
-__device__ __forceinline__ Work locate(const Attn &a, uint32_t id, bool by_seq, bool report, Count count) {
+__device__ __forceinline__ Work locate(const Attn &a, uint32_t id, bool by_seq, Count count) {
     const uint32_t lane = threadIdx.x & 63u;
     Work w;
     w.seq = -1;
     uint32_t before = 0;
     for (uint32_t base = 0; base < a.b.n_seq; base += 64) {
         int len, t0, n;
-        load_seq(a, base, report, len, t0, n);
+        load_seq(a, base, false, len, t0, n);
         const uint32_t c = n > 0 ? count(len, n) : 0u;
-        uint32_t sum = c;   // inclusive over the lanes
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t p = (uint32_t)__shfl_up((int)sum, o, 64);
-            if (lane >= (uint32_t)o) sum += p;
-        }
-        const uint32_t lo = before + sum - c;
+        const uint32_t sum = wave_scan_u32(c), lo = before + sum - c;
         const bool mine = c > 0 && (by_seq ? base + lane == id : id >= lo && id < lo + c);
         const uint64_t m = __builtin_amdgcn_ballot_w64(mine);
-        if (m != 0 && w.seq < 0) {
+        if (m != 0) {
             const int l = __builtin_ctzll(m);
             w.seq = (int)base + l;
             w.len = __builtin_amdgcn_readlane(len, l);
             w.tok0 = __builtin_amdgcn_readlane(t0, l);
             w.n_new = __builtin_amdgcn_readlane(n, l);
             w.first = (uint32_t)__builtin_amdgcn_readlane((int)lo, l);
+            w.count = (uint32_t)__builtin_amdgcn_readlane((int)c, l);
             w.item = by_seq ? 0u : id - w.first;
-            if (!report) return w;
+            return w;
         }
         before += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
     }
     return w;
 }
+// raise the error of lengths over the bounds
+__device__ __forceinline__ void report_lengths(const Attn &a) {
+    for (uint32_t base = 0; base < a.b.n_seq; base += 64) {
+        int len, t0, n;
+        load_seq(a, base, true, len, t0, n);
+    }
+}
 
 __device__ __forceinline__ bool is_split(const Attn &a, int n) { return (uint32_t)n * a.gqa <= a.split_rows; }
 
-// kv4_split_kernel's chunks: ct tiles of rows each, the smallest ct for which
-// all of them fit the launch's slots (sum of ceil(tiles / ct) <= tiles /
-// (n_slots - n_seq) + n_seq); a sequence with tokens has at least one.
+// kv4_split_kernel's work is the list of its sequences' tiles, one sequence
+// after the other (at least one each), in equal shares: slot i takes tiles [i
+// ct, (i + 1) ct), except that a sequence of up to WHOLE tiles goes undivided
+// to the slot of its first.
 __device__ __forceinline__ uint32_t tiles_of(const Attn &a, int len, int n) {
     return is_split(a, n) ? max(1u, (min((uint32_t)len, row_cap(a)) + TILE - 1u) / TILE) : 0u;
 }
-__device__ __forceinline__ uint32_t chunk_tiles(const Attn &a) {
+__device__ __forceinline__ uint32_t all_tiles(const Attn &a) {
     uint32_t total = 0;
     for (uint32_t base = 0; base < a.b.n_seq; base += 64) {
         int len, t0, n;
         load_seq(a, base, false, len, t0, n);
-        uint32_t v = n > 0 ? tiles_of(a, len, n) : 0u;
-        v += (uint32_t)dpp_i<DPP_XOR1>((int)v);
-        v += (uint32_t)dpp_i<DPP_XOR2>((int)v);
-        v += (uint32_t)dpp_i<DPP_HALF_MIRROR>((int)v);
-        v += (uint32_t)dpp_i<DPP_MIRROR>((int)v);
-#pragma unroll
-        for (int r = 0; r < 4; r++) total += (uint32_t)__builtin_amdgcn_readlane((int)v, 16 * r);
+        total += (uint32_t)__builtin_amdgcn_readlane((int)wave_scan_u32(n > 0 ? tiles_of(a, len, n) : 0u), 63);
     }
-    const uint32_t room = a.n_slots - a.b.n_seq;
-    return max(CT_MIN, room ? (total + room - 1u) / room : 0x7fffffu);
+    return total;
 }
-__device__ __forceinline__ Work find_chunk(const Attn &a, uint32_t ct, uint32_t id, bool by_seq, bool report) {
-    return locate(a, id, by_seq, report, [&](int len, int n) { return (tiles_of(a, len, n) + ct - 1u) / ct; });
+__device__ __forceinline__ uint32_t slot_tiles(const Attn &a, uint32_t total) {
+    return max(CT_MIN, (total + a.n_slots - 1u) / a.n_slots);
+}
+__device__ __forceinline__ Work find_tiles(const Attn &a, uint32_t id, bool by_seq) {
+    return locate(a, id, by_seq, [&](int len, int n) { return tiles_of(a, len, n); });
 }
 
 // the gated, normalised output of four elements
@@ -440,9 +457,9 @@ __device__ __forceinline__ f16x8 join8(f16x2 a, f16x2 b, f16x2 c, f16x2 d) {
 // largest scale seen, 2^dlog; a new reference leaves the largest at 2^FRESH.
 constexpr float TOP = 15.0f, FRESH = 6.0f;
 
-// Work item: (chunk slot, kv head, tile of 16 rows), a row being a (token, q
-// head of the group) pair, token-major.  Each wave streams its own 32-row
-// tiles of the chunk (every fourth) through a private double buffer filled by
+// Work item: (slot, kv head, tile of 16 rows), a row being a (token, q head of
+// the group) pair, token-major; the slot's sequences one after the other.
+// Each wave streams its own 32-row tiles of a segment (every fourth) through a private double buffer filled by
 // LDS-DMA, so that no barrier stands between the first tile and the last.
 //
 // Scores S^T = K Q^T on 16x16x32 f16 MFMA, one per block of 32 dims: the codes
@@ -464,68 +481,26 @@ __global__ __launch_bounds__(256, 2) void kv4_split_kernel(Attn a) {
     const uint32_t r16 = lane & 15u, g4 = lane >> 4, NKV = a.b.nkv;
     const uint32_t per = a.n_slots * NKV, mt = blockIdx.x / per, it = blockIdx.x % per;
     const uint32_t g = it % NKV, slot = it / NKV;
-    const uint32_t ct = chunk_tiles(a);
-    const Work wk = find_chunk(a, ct, slot, false, blockIdx.x == 0 && w == 0);
-    if (wk.seq < 0) return;
+    const uint32_t total = all_tiles(a), ct = slot_tiles(a, total), x0 = slot * ct, x1 = min(x0 + ct, total);
+    bool again = false;
+    for (uint32_t x = x0; x < x1;) {
+    const Work wk = find_tiles(a, x, false);
+    if (wk.seq < 0) break;   // (never: x < total)
+    const uint32_t t0 = x - wk.first, t1 = wk.count <= WHOLE ? wk.count : min(x1 - wk.first, wk.count);   // its tiles here
+    const bool ours = t0 == 0 || wk.count > WHOLE, whole = t0 == 0 && t1 == wk.count;
+    const uint32_t rec0 = slot * 2 + (x > x0 ? 1u : 0u);
+    x = wk.first + t1;
     const uint32_t M = (uint32_t)wk.n_new * a.gqa;
-    if (16 * mt >= M) return;
+    if (!ours || 16 * mt >= M) continue;
+    if (again) __syncthreads();   // (the last segment's sums have been read)
+    again = true;
     const uint32_t rows = min(16u, M - 16 * mt);
     const int p0 = wk.len - wk.n_new;   // the first token's position
     auto row_pos = [&](uint32_t r) { return p0 + (int)((16 * mt + r) / a.gqa); };
-    const int pmin = row_pos(0), pmax = row_pos(rows - 1), c0 = (int)(wk.item * ct * TILE);
-    if (wk.item > 0 && c0 > pmax) return;
-    const int cap = (int)row_cap(a);
-    const int end = min(min(c0 + (int)(ct * TILE), pmax + 1), cap);   // rows [c0, end)
+    const int pmin = row_pos(0), pmax = row_pos(rows - 1), c0 = (int)(t0 * TILE), cap = (int)row_cap(a);
+    const int end = min(min((int)(t1 * TILE), pmax + 1), cap);            // rows [c0, end)
     const int my_vis = r16 < rows ? min(row_pos(r16) + 1, end) : end;     // of them this lane's row sees [c0, my_vis)
     const int n_tile = end > c0 ? (end - c0 + (int)TILE - 1) / (int)TILE : 0;
-
-    // the row's q: dims 32 b + {4 g, .., 4 g + 3} and 16 further, in the codes' order
-    f16x8 Q[NS][NB];
-    float qs;
-    {
-        const uint32_t r = 16 * mt + min(r16, rows - 1);
-        const int64_t e0 = (int64_t)(wk.tok0 + (int)(r / a.gqa)) * a.q.ld + (int64_t)(g * a.gqa + r % a.gqa) * a.q.hs + 4 * g4;
-        float4 x[2 * NB];
-        float am = 0.0f;
-        // (all loads in flight before the first is used: no branch on the type between them)
-        if constexpr (NS == 2) {
-#pragma unroll
-            for (uint32_t b = 0; b < 2 * NB; b++)
-                x[b] = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q.p) + e0 + 16 * b);
-        } else {
-            u32x2 u[2 * NB];
-#pragma unroll
-            for (uint32_t b = 0; b < 2 * NB; b++)
-                u[b] = *reinterpret_cast<const u32x2 *>(static_cast<const uint16_t *>(a.q.p) + e0 + 16 * b);
-            const bool bf = a.type == SINTER_BF16;
-#pragma unroll
-            for (uint32_t b = 0; b < 2 * NB; b++) {
-                const float4 m = cvt4(u[b], SINTER_BF16), n = cvt4(u[b], SINTER_F16);
-                x[b] = make_float4(bf ? m.x : n.x, bf ? m.y : n.y, bf ? m.z : n.z, bf ? m.w : n.w);
-            }
-        }
-#pragma unroll
-        for (uint32_t b = 0; b < 2 * NB; b++)
-            am = fmaxf(am, fmaxf(fmaxf(fabsf(x[b].x), fabsf(x[b].y)), fmaxf(fabsf(x[b].z), fabsf(x[b].w))));
-        am = fmaxf(am, __shfl_xor(am, 16, 64));
-        am = fmaxf(am, __shfl_xor(am, 32, 64));
-        // the row's largest element to [2^13, 2^14): its scale is a power of two
-        int ex = am > 0.0f && am < INFINITY ? 14 - (int)((__float_as_uint(fmaxf(am, 1e-30f)) >> 23) - 126u) : 0;
-        const float up = r16 < rows ? ldexpf(1.0f, ex) : 0.0f;
-        qs = a.qscale * ldexpf(1.0f, -ex);
-#pragma unroll
-        for (uint32_t b = 0; b < NB; b++) {
-            const float4 l = x[2 * b], h = x[2 * b + 1];
-            float f[8] = {l.x * up, l.z * up, l.y * up, l.w * up, h.x * up, h.z * up, h.y * up, h.w * up};
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                if constexpr (NS == 2) asm volatile("" : "+v"(f[i]));   // (as for the weights below)
-                const _Float16 hi = (_Float16)f[i];
-                Q[0][b][i] = hi;
-                if constexpr (NS == 2) Q[NS - 1][b][i] = (_Float16)(f[i] - (float)hi);
-            }
-        }
-    }
 
     LDS unsigned char *L = (LDS unsigned char *)sm + w * 2 * STAGE;
     const uint32_t lbase = (uint32_t)(uintptr_t)(LDS unsigned char *)sm + w * 2 * STAGE;
@@ -584,13 +559,61 @@ __global__ __launch_bounds__(256, 2) void kv4_split_kernel(Attn a) {
         }
     };
 
+    const int nt = (n_tile - (int)w + 3) / 4;
+    if (nt > 0) issue((int)w, 0);
+    // the row's q, while the first tile is on its way: dims 32 b + {4 g, .., 4 g + 3} and 16 further, in the codes' order
+    f16x8 Q[NS][NB];
+    float qs;
+    {
+        const uint32_t r = 16 * mt + min(r16, rows - 1);
+        const int64_t e0 = (int64_t)(wk.tok0 + (int)(r / a.gqa)) * a.q.ld + (int64_t)(g * a.gqa + r % a.gqa) * a.q.hs + 4 * g4;
+        float4 x[2 * NB];
+        float am = 0.0f;
+        // (all loads in flight before the first is used: no branch on the type between them)
+        if constexpr (NS == 2) {
+#pragma unroll
+            for (uint32_t b = 0; b < 2 * NB; b++)
+                x[b] = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q.p) + e0 + 16 * b);
+        } else {
+            u32x2 u[2 * NB];
+#pragma unroll
+            for (uint32_t b = 0; b < 2 * NB; b++)
+                u[b] = *reinterpret_cast<const u32x2 *>(static_cast<const uint16_t *>(a.q.p) + e0 + 16 * b);
+            const bool bf = a.type == SINTER_BF16;
+#pragma unroll
+            for (uint32_t b = 0; b < 2 * NB; b++) {
+                const float4 m = cvt4(u[b], SINTER_BF16), n = cvt4(u[b], SINTER_F16);
+                x[b] = make_float4(bf ? m.x : n.x, bf ? m.y : n.y, bf ? m.z : n.z, bf ? m.w : n.w);
+            }
+        }
+#pragma unroll
+        for (uint32_t b = 0; b < 2 * NB; b++)
+            am = fmaxf(am, fmaxf(fmaxf(fabsf(x[b].x), fabsf(x[b].y)), fmaxf(fabsf(x[b].z), fabsf(x[b].w))));
+        am = fmaxf(am, __shfl_xor(am, 16, 64));
+        am = fmaxf(am, __shfl_xor(am, 32, 64));
+        // the row's largest element to [2^13, 2^14): its scale is a power of two
+        int ex = am > 0.0f && am < INFINITY ? 14 - (int)((__float_as_uint(fmaxf(am, 1e-30f)) >> 23) - 126u) : 0;
+        const float up = r16 < rows ? ldexpf(1.0f, ex) : 0.0f;
+        qs = a.qscale * ldexpf(1.0f, -ex);
+#pragma unroll
+        for (uint32_t b = 0; b < NB; b++) {
+            const float4 l = x[2 * b], h = x[2 * b + 1];
+            float f[8] = {l.x * up, l.z * up, l.y * up, l.w * up, h.x * up, h.z * up, h.y * up, h.w * up};
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                if constexpr (NS == 2) asm volatile("" : "+v"(f[i]));   // (as for the weights below)
+                const _Float16 hi = (_Float16)f[i];
+                Q[0][b][i] = hi;
+                if constexpr (NS == 2) Q[NS - 1][b][i] = (_Float16)(f[i] - (float)hi);
+            }
+        }
+    }
+
     f32x4 O[2 * NB];
 #pragma unroll
     for (uint32_t i = 0; i < 2 * NB; i++) O[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     float ref = REF_NONE, lim = REF_NONE, lsum = 0.0f;
     float dtop = 0.0f, dlog = -24.0f;   // every V scale so far is at most dtop = 2^dlog (dtop 0: none yet)
-    const int nt = (n_tile - (int)w + 3) / 4;
-    if (nt > 0) issue((int)w, 0);
     for (int i = 0; i < nt; i++) {
         const uint32_t st = i & 1;
         // (opaque, as in issue)
@@ -758,65 +781,69 @@ __global__ __launch_bounds__(256, 2) void kv4_split_kernel(Attn a) {
 #pragma unroll
             for (int j = 0; j < 4; j++) o[j] = fmaf(x[j], c, o[j]);
         }
-        const int pos = min(row_pos(r), cap - 1);   // (cap: rows the launch and the table have room for)
-        if (pos < c0 && wk.item > 0) continue;   // (the row ends before this chunk)
-        if (pos < (int)(ct * TILE)) {   // the row sees chunk 0 alone
+        if (whole) {
             store_out(a, wk.tok0 + (int)((16 * mt + r) / a.gqa), g * a.gqa + (16 * mt + r) % a.gqa, e, o, l);
         } else {
-            const size_t rec = (((size_t)slot * NKV + g) * a.n_mt + mt) * 16 + r;
+            const size_t rec = (((size_t)rec0 * NKV + g) * a.n_mt + mt) * 16 + r;
             *reinterpret_cast<f32x4 *>(a.part + rec * HD + e) = o;
             if (e == 0) a.ml[rec] = make_float2(m, l);
         }
     }
+    }
+    if (blockIdx.x == 0 && w == 0) report_lengths(a);
 }
 
-// A row that sees more than one chunk: out = sum c_i O_i / sum c_i l_i with
-// c_i = exp2(ref_i - max ref).  One workgroup per (sequence, kv head, row);
-// wave w takes every fourth chunk.
-__global__ __launch_bounds__(256) void kv4_merge_kernel(Attn a, uint32_t rows) {
-    __shared__ float red[2][4];
-    __shared__ __attribute__((aligned(16))) float comb[4][256];
+// A sequence divided over slots: out = sum c_i O_i / sum c_i l_i with c_i =
+// exp2(ref_i - max ref) over its segments.  One workgroup per (sequence, kv
+// head, row); wave w takes every NW-th segment, all of its loads in flight for
+// up to 8 NW.
+template <int NW>
+__global__ __launch_bounds__(64 * NW) void kv4_merge_kernel(Attn a, uint32_t rows) {
+    __shared__ float red[NW];
+    __shared__ __attribute__((aligned(16))) float comb[NW][256];
     const uint32_t r = blockIdx.x % rows, sg = blockIdx.x / rows, g = sg % a.b.nkv, lane = threadIdx.x & 63u, HD = a.b.hd;
     const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t ct = chunk_tiles(a);
-    const Work wk = find_chunk(a, ct, sg / a.b.nkv, true, false);
-    if (wk.seq < 0) return;
-    const uint32_t i = r / a.gqa, h = g * a.gqa + r % a.gqa, t = (uint32_t)wk.tok0 + i, span = ct * TILE;
-    const int pos = min(wk.len - wk.n_new + (int)i, (int)row_cap(a) - 1);
-    if (i >= (uint32_t)wk.n_new || pos < (int)span) return;
-    const uint32_t n = (uint32_t)pos / span + 1u;   // chunks the row sees
-    auto rec = [&](uint32_t c) { return (((size_t)(wk.first + c) * a.b.nkv + g) * a.n_mt + r / 16) * 16 + r % 16; };
+    const Work wk = find_tiles(a, sg / a.b.nkv, true);
+    if (wk.seq < 0 || wk.count <= WHOLE || r >= (uint32_t)wk.n_new * a.gqa) return;
+    const uint32_t ct = slot_tiles(a, all_tiles(a)), i0 = wk.first / ct, i1 = (wk.first + wk.count - 1u) / ct;
+    if (i0 == i1) return;
+    const uint32_t n = i1 - i0 + 1u, head1 = wk.first > i0 * ct ? 1u : 0u;   // (its first segment: the slot's own first, or its last)
+    auto rec = [&](uint32_t c) {
+        return (((size_t)((i0 + c) * 2 + (c == 0 ? head1 : 0u)) * a.b.nkv + g) * a.n_mt + r / 16) * 16 + r % 16;
+    };
     float m = REF_NONE, l = 0.0f;
     for (uint32_t c = lane; c < n; c += 64) m = fmaxf(m, a.ml[rec(c)].x);
     m = wave_max_f32(m);
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
     const uint32_t e = 4 * lane;
-    for (uint32_t c0 = w; c0 < n; c0 += 32) {
+    for (uint32_t c0 = w; c0 < n; c0 += 8 * NW) {
         f32x4 x[8];
         float2 ml[8];
 #pragma unroll
         for (uint32_t k = 0; k < 8; k++) {
-            const size_t at = rec(min(c0 + 4 * k, n - 1u));
+            const size_t at = rec(min(c0 + NW * k, n - 1u));
             ml[k] = a.ml[at];
             x[k] = *reinterpret_cast<const f32x4 *>(a.part + at * HD + (e < HD ? e : 0u));
         }
 #pragma unroll
         for (uint32_t k = 0; k < 8; k++) {
-            if (c0 + 4 * k >= n) break;
+            if (c0 + NW * k >= n) break;
             const float c = __builtin_amdgcn_exp2f(ml[k].x - m);
             l = fmaf(ml[k].y, c, l);
 #pragma unroll
             for (int j = 0; j < 4; j++) o[j] = fmaf(x[k][j], c, o[j]);
         }
     }
-    if (lane == 0) red[0][w] = l;
+    if (lane == 0) red[w] = l;
     *reinterpret_cast<f32x4 *>(&comb[w][e]) = o;
     __syncthreads();
     if (w != 0 || e >= HD) return;
-    l = (red[0][0] + red[0][1]) + (red[0][2] + red[0][3]);
 #pragma unroll
-    for (uint32_t k = 1; k < 4; k++) o = o + *reinterpret_cast<const f32x4 *>(&comb[k][e]);
-    store_out(a, t, h, e, o, l);
+    for (uint32_t k = 1; k < NW; k++) {
+        l += red[k];
+        o = o + *reinterpret_cast<const f32x4 *>(&comb[k][e]);
+    }
+    store_out(a, wk.tok0 + (int)(r / a.gqa), g * a.gqa + r % a.gqa, e, o, l);
 }
 
 // ------------------------------------------------------------------ many rows
@@ -824,31 +851,22 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(Attn a, uint32_t rows) {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 // the tiles of ROWS rows of sequences that kv4_split_kernel leaves out
-__device__ __forceinline__ Work find_tile(const Attn &a, uint32_t rows, uint32_t id, bool by_seq, bool report) {
-    return locate(a, id, by_seq, report, [&](int len, int n) {
+__device__ __forceinline__ Work find_tile(const Attn &a, uint32_t rows, uint32_t id, bool by_seq) {
+    return locate(a, id, by_seq, [&](int len, int n) {
         return is_split(a, n) ? 0u : ((uint32_t)n * a.gqa + rows - 1u) / rows;
     });
 }
-__device__ __forceinline__ uint32_t wave_sum_u32(uint32_t v) {
-    v += (uint32_t)dpp_i<DPP_XOR1>((int)v);
-    v += (uint32_t)dpp_i<DPP_XOR2>((int)v);
-    v += (uint32_t)dpp_i<DPP_HALF_MIRROR>((int)v);
-    v += (uint32_t)dpp_i<DPP_MIRROR>((int)v);
-    uint32_t t = 0;
-#pragma unroll
-    for (int r = 0; r < 4; r++) t += (uint32_t)__builtin_amdgcn_readlane((int)v, 16 * r);
-    return t;
-}
+__device__ __forceinline__ uint32_t wave_sum_u32(uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)wave_scan_u32(v), 63); }
 // The id-th tile from the one with the most cache rows down, so that the
 // longest start first (two prompts of 2000 tokens, bf16, 27B heads: sequence
 // after sequence 377 us, so 205).  A sequence with p0 rows before its tokens
 // has one tile in each of the levels p0 gqa / rows + 0, 1, ..: the level is
 // found by bisection over the count of tiles at or above it, a lane a
 // sequence.  More than 64 sequences are taken in their order.
-__device__ __forceinline__ Work find_ranked_tile(const Attn &a, uint32_t rows, uint32_t id, bool report) {
-    if (a.b.n_seq > 64) return find_tile(a, rows, id, false, report);
+__device__ __forceinline__ Work find_ranked_tile(const Attn &a, uint32_t rows, uint32_t id) {
+    if (a.b.n_seq > 64) return find_tile(a, rows, id, false);
     int len, t0, n;
-    load_seq(a, 0, report, len, t0, n);
+    load_seq(a, 0, false, len, t0, n);
     const uint32_t c = n > 0 && !is_split(a, n) ? ((uint32_t)n * a.gqa + rows - 1u) / rows : 0u;
     const uint32_t base = (uint32_t)((uint64_t)(uint32_t)max(0, len - n) * a.gqa / rows), top = c ? base + c : 0u;
     // (no branch on c: every lane takes part in the sums)
@@ -931,7 +949,8 @@ __global__ __launch_bounds__(64 * NW, T == SINTER_F32 ? 1 : 2) void kv4_tile_ker
     const uint32_t g = id % NKV;
     id /= NKV;
     const uint32_t ck = id / a.n_tile;
-    const Work wk = find_ranked_tile(a, ROWS, id % a.n_tile, a.report && blockIdx.x == 0 && w == 0);
+    if (a.report && blockIdx.x == 0 && w == 0) report_lengths(a);
+    const Work wk = find_ranked_tile(a, ROWS, id % a.n_tile);
     if (wk.seq < 0) return;
     const uint32_t gt = wk.first + wk.item;
     const uint32_t M = (uint32_t)wk.n_new * a.gqa, r0 = wk.item * ROWS;
@@ -1368,7 +1387,7 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Attn a) {
     const uint32_t t = u / a.nq, h = u % a.nq;
     const int seq = seq_of(a.b, t);
     if (seq < 0) return;
-    const Work wk = find_tile(a, ROWS, (uint32_t)seq, true, false);
+    const Work wk = find_tile(a, ROWS, (uint32_t)seq, true);
     if (wk.seq < 0) return;
     const uint32_t i = t - (uint32_t)wk.tok0;
     if (i >= (uint32_t)wk.n_new || i >= a.max_q) return;
@@ -1453,10 +1472,10 @@ int check_attn(const sinter_kv4_batch *b, const sinter_kv4_attn_args *a) {
 // bf16: 684 us against 587)
 constexpr uint32_t tile_waves(bool f32) { return f32 ? 4 : 8; }
 
-// The launches of a batch.  kv4_split_kernel: row tiles a sequence and chunk
-// slots, a slot a sequence and, where there may be rows to split, as many more
-// as give every CU some workgroups.  kv4_tile_kernel: row tiles (at most one
+// The launches of a batch.  kv4_split_kernel: row tiles a sequence, and slots,
+// as many as run at once (two workgroups a CU).  kv4_tile_kernel: row tiles (at most one
 // partly filled one a sequence) and chunks of the cache rows a tile sees.
+constexpr uint32_t SLOTS = 512;
 struct Plan {
     uint32_t n_mt = 0, n_slots = 0, n_tile = 0, n_split = 1;
     bool split = false, merge = false, join = false;
@@ -1473,15 +1492,12 @@ Plan make_plan(const sinter_kv4_batch &b, const sinter_kv4_attn_args &a) {
     p.split = gqa <= SPLIT_ROWS && (rows <= SPLIT_ROWS || b.n_seq > 1);
     if (p.split) {
         p.n_mt = (uint32_t)((std::min<uint64_t>(rows, SPLIT_ROWS) + 15) / 16);
-        p.merge = a.max_kv > CT_MIN * TILE;
-        p.n_slots = b.n_seq;
-        if (p.merge) {
-            const uint64_t per = (uint64_t)b.nkv * p.n_mt;
-            const uint64_t most = (uint64_t)b.n_seq * ((a.max_kv + CT_MIN * TILE - 1) / (CT_MIN * TILE));
-            p.n_slots += (uint32_t)std::min<uint64_t>(std::max<uint64_t>(1, 1024 / per), most);
-        }
+        p.merge = a.max_kv > WHOLE * TILE;
+        const uint64_t per = (uint64_t)b.nkv * p.n_mt;
+        const uint64_t most = (uint64_t)b.n_seq * std::max<uint64_t>(1, (a.max_kv + CT_MIN * TILE - 1) / (CT_MIN * TILE));
+        p.n_slots = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(1, SLOTS / per), most);
         p.grid = (uint64_t)p.n_slots * b.nkv * p.n_mt;
-        p.recs = p.merge ? (size_t)p.grid * 16 : 0;
+        p.recs = p.merge ? (size_t)p.grid * 32 : 0;
     }
     if (!p.split || rows > SPLIT_ROWS) {
         const uint64_t least = p.split ? SPLIT_ROWS / gqa + 1 : 1;   // tokens of a sequence that comes here
@@ -1659,7 +1675,10 @@ int sinter_kv4_attn(const sinter_kv4_batch *b, const sinter_kv4_attn_args *a, vo
     }
     if (p.merge) {
         const uint32_t rows = std::min(std::min(a->max_q, b->n_tok) * k.gqa, SPLIT_ROWS / k.gqa * k.gqa);
-        hipLaunchKernelGGL(kv4_merge_kernel, dim3(b->n_seq * b->nkv * rows), dim3(256), 0, s, k, rows);
+        const uint32_t grid = b->n_seq * b->nkv * rows;
+        // (few rows over many slots: a wave a segment or two)
+        if (p.n_slots > 32 * b->n_seq) hipLaunchKernelGGL((kv4_merge_kernel<16>), dim3(grid), dim3(1024), 0, s, k, rows);
+        else hipLaunchKernelGGL((kv4_merge_kernel<4>), dim3(grid), dim3(256), 0, s, k, rows);
     }
     return hip_ok(hipGetLastError(), "kv4_attn: merge launch") ? SINTER_OK : SINTER_ERR_HIP;
 }
