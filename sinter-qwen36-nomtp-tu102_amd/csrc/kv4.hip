@@ -279,6 +279,7 @@ struct Attn {
     uint32_t nq, gqa, max_q, max_kv, n_slots, n_mt, type, page_shift;
     uint32_t n_tile, n_split, report;   // kv4_tile_kernel: row tiles and chunks; report the errors of lengths
     uint32_t split_rows;   // sequences of up to these rows are kv4_split_kernel's (SPLIT_ROWS; 0: it is not launched)
+    uint32_t gqa_inv;   // ceil(2^32 / gqa), gqa > 1
     float qscale;    // scale * log2(e)
 };
 
@@ -479,8 +480,9 @@ __global__ __launch_bounds__(256, 2) void kv4_split_kernel(Attn a) {
     __shared__ float red[2][4][16];
     const uint32_t lane = threadIdx.x & 63u, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t r16 = lane & 15u, g4 = lane >> 4, NKV = a.b.nkv;
-    const uint32_t per = a.n_slots * NKV, mt = blockIdx.x / per, it = blockIdx.x % per;
-    const uint32_t g = it % NKV, slot = it / NKV;
+    const uint32_t g = blockIdx.x, slot = blockIdx.y, mt = blockIdx.z;
+    // (a row's token: rows < 32, gqa <= 32, so the product with ceil(2^32 / gqa) has the quotient)
+    auto tok_of = [&](uint32_t r) { return a.gqa == 1 ? 16 * mt + r : __umulhi(16 * mt + r, a.gqa_inv); };
     const uint32_t total = all_tiles(a), ct = slot_tiles(a, total), x0 = slot * ct, x1 = min(x0 + ct, total);
     bool again = false;
     for (uint32_t x = x0; x < x1;) {
@@ -496,7 +498,7 @@ __global__ __launch_bounds__(256, 2) void kv4_split_kernel(Attn a) {
     again = true;
     const uint32_t rows = min(16u, M - 16 * mt);
     const int p0 = wk.len - wk.n_new;   // the first token's position
-    auto row_pos = [&](uint32_t r) { return p0 + (int)((16 * mt + r) / a.gqa); };
+    auto row_pos = [&](uint32_t r) { return p0 + (int)tok_of(r); };
     const int pmin = row_pos(0), pmax = row_pos(rows - 1), c0 = (int)(t0 * TILE), cap = (int)row_cap(a);
     const int end = min(min((int)(t1 * TILE), pmax + 1), cap);            // rows [c0, end)
     const int my_vis = r16 < rows ? min(row_pos(r16) + 1, end) : end;     // of them this lane's row sees [c0, my_vis)
@@ -565,8 +567,8 @@ __global__ __launch_bounds__(256, 2) void kv4_split_kernel(Attn a) {
     f16x8 Q[NS][NB];
     float qs;
     {
-        const uint32_t r = 16 * mt + min(r16, rows - 1);
-        const int64_t e0 = (int64_t)(wk.tok0 + (int)(r / a.gqa)) * a.q.ld + (int64_t)(g * a.gqa + r % a.gqa) * a.q.hs + 4 * g4;
+        const uint32_t r = min(r16, rows - 1), tk = tok_of(r);
+        const int64_t e0 = (int64_t)(wk.tok0 + (int)tk) * a.q.ld + (int64_t)((g - tk) * a.gqa + 16 * mt + r) * a.q.hs + 4 * g4;
         float4 x[2 * NB];
         float am = 0.0f;
         // (all loads in flight before the first is used: no branch on the type between them)
@@ -633,34 +635,60 @@ __global__ __launch_bounds__(256, 2) void kv4_split_kernel(Attn a) {
         }
         const int row0 = c0 + ((int)w + 4 * i) * (int)TILE;
         const LDS unsigned char *kt = L + st * STAGE, *vt = kt + KC, *ks = kt + 2 * KC, *vs = ks + SC;
-        float s[2][4];
+        // Scores, step by step kept in this order: a block's codes are taken
+        // apart while the block before it is on the matrix core, whose sums are
+        // scaled a step later (left to the scheduler each step waits for its
+        // read, its MFMA and its sums in turn: 7000 cycles a tile of F32 rows)
+        float s[2][4] = {};
+        uint32_t kx[2][NB], d[2][4][NB / 2];   // codes; scales of keys 4 g + v, two blocks a word
 #pragma unroll
         for (uint32_t h = 0; h < 2; h++) {
-            sched_fence();
-            uint32_t d[4][NB / 2];   // scales of keys 4 g + v, two blocks a word
+            const uint32_t r = 16 * h + r16;
+#pragma unroll
+            for (uint32_t b = 0; b < NB; b++)
+                kx[h][b] = *reinterpret_cast<const LDS uint32_t *>(kt + r * HB + 16 * (b ^ swz(r)) + 4 * g4);
 #pragma unroll
             for (uint32_t v = 0; v < 4; v++)
 #pragma unroll
                 for (uint32_t b = 0; b < NB / 2; b++)
-                    d[v][b] = reinterpret_cast<const LDS uint32_t *>(ks + (16 * h + 4 * g4 + v) * SB)[b];
+                    d[h][v][b] = reinterpret_cast<const LDS uint32_t *>(ks + (16 * h + 4 * g4 + v) * SB)[b];
+        }
+        auto k_operand = [&](uint32_t u) {
+            const uint32_t x = kx[u / NB][u % NB];
+            return join8(code_pair_lo(x), code_pair_lo(x >> 8), code_pair_hi(x), code_pair_hi(x >> 8));
+        };
+        f16x8 A = k_operand(0);
+        f32x4 t[2];
+        auto scaled = [&](uint32_t u) {
+            const uint32_t h = u / NB, b = u % NB;
 #pragma unroll
-            for (uint32_t v = 0; v < 4; v++) s[h][v] = 0.0f;
-            const uint32_t r = 16 * h + r16;
-#pragma unroll
-            for (uint32_t b = 0; b < NB; b++) {
-                const uint32_t x = *reinterpret_cast<const LDS uint32_t *>(kt + r * HB + 16 * (b ^ swz(r)) + 4 * g4);
-                const f16x8 A = join8(code_pair_lo(x), code_pair_lo(x >> 8), code_pair_hi(x), code_pair_hi(x >> 8));
-                f32x4 t = {0.0f, 0.0f, 0.0f, 0.0f};
-                t = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, Q[0][b], t, 0, 0, 0);
-                if constexpr (NS == 2) t = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, Q[NS - 1][b], t, 0, 0, 0);
-#pragma unroll
-                for (uint32_t v = 0; v < 4; v++) {
-                    const f16x2 dd = pair_of(d[v][b / 2]);
-                    s[h][v] = fmaf(t[v], (float)(b & 1 ? dd.y : dd.x), s[h][v]);
-                }
+            for (uint32_t v = 0; v < 4; v++) {
+                const f16x2 dd = pair_of(d[h][v][b / 2]);
+                s[h][v] = fmaf(t[u & 1][v], (float)(b & 1 ? dd.y : dd.x), s[h][v]);
             }
+        };
+#pragma unroll
+        for (uint32_t u = 0; u < 2 * NB; u++) {
+            sched_fence();
+            const f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
+            t[u & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, Q[0][u % NB], z, 0, 0, 0);
+            if constexpr (NS == 2) t[u & 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, Q[NS - 1][u % NB], t[u & 1], 0, 0, 0);
+            if (u + 1 < 2 * NB) A = k_operand(u + 1);
+            if (u > 0) scaled(u - 1);
         }
         sched_fence();
+        // V's codes and scales, on their way while the weights are made
+        const uint32_t kr = (r16 >> 1), vr = 16 * (kr >> 2) + 4 * g4 + (kr & 3);
+        auto v_codes = [&](uint32_t b) {
+            // (lane i of a group of 16 reads half i % 2 of row key(i / 2) and
+            // gets byte i of the block for the group's eight keys)
+            return __builtin_amdgcn_ds_read_tr8_b64_v2i32((LDS i32x2 *)(vt + vr * HB + 16 * (b ^ swz(vr)) + 8 * (r16 & 1u)));
+        };
+        i32x2 vx[NB];
+        constexpr uint32_t AHEAD = NS == 2 && NB == 8 ? 4 : NB;
+#pragma unroll
+        for (uint32_t b = 0; b < AHEAD; b++) vx[b] = v_codes(b);
+        scaled(2 * NB - 1);
         uint32_t dv[8][NB / 2];
 #pragma unroll
         for (uint32_t k = 0; k < 8; k++)
@@ -720,18 +748,12 @@ __global__ __launch_bounds__(256, 2) void kv4_split_kernel(Attn a) {
             p[k] = __builtin_amdgcn_exp2f(fmaf(p[k], qs, -ref));   // (0 where masked)
             lsum += p[k];
         }
-        // V^T: lane i of a group of 16 reads half i % 2 of row key(i / 2) and
-        // gets byte i of the block for the group's eight keys
-        const uint32_t kr = (r16 >> 1), vr = 16 * (kr >> 2) + 4 * g4 + (kr & 3);
-#pragma unroll
-        for (uint32_t b = 0; b < NB; b++) {
-            if (NS == 2 || b % 2 == 0) sched_fence();
-            const i32x2 x = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                (LDS i32x2 *)(vt + vr * HB + 16 * (b ^ swz(vr)) + 8 * (r16 & 1u)));
-            const uint32_t x0 = (uint32_t)x.x, x1 = (uint32_t)x.y;
-            const f16x8 Al = join8(code_pair_lo(x0), code_pair_lo(x0 >> 8), code_pair_lo(x1), code_pair_lo(x1 >> 8));
-            const f16x8 Ah = join8(code_pair_hi(x0), code_pair_hi(x0 >> 8), code_pair_hi(x1), code_pair_hi(x1 >> 8));
-            f16x8 P, Pl;
+        // The sums, in the same way
+        f16x8 Al, Ah, P, Pl;
+        auto v_operands = [&](uint32_t b) {
+            const uint32_t x0 = (uint32_t)vx[b].x, x1 = (uint32_t)vx[b].y;
+            Al = join8(code_pair_lo(x0), code_pair_lo(x0 >> 8), code_pair_lo(x1), code_pair_lo(x1 >> 8));
+            Ah = join8(code_pair_hi(x0), code_pair_hi(x0 >> 8), code_pair_hi(x1), code_pair_hi(x1 >> 8));
 #pragma unroll
             for (uint32_t k = 0; k < 8; k += 2) {   // keys 0 2, 1 3, 4 6, 5 7
                 const uint32_t k0 = (k & 4) | ((k >> 1) & 1), k1 = k0 + 2;
@@ -747,13 +769,21 @@ __global__ __launch_bounds__(256, 2) void kv4_split_kernel(Attn a) {
                     Pl[k] = lo.x; Pl[k + 1] = lo.y;
                 }
             }
+        };
+        v_operands(0);
+#pragma unroll
+        for (uint32_t b = 0; b < NB; b++) {
+            sched_fence();
             O[2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(Al, P, O[2 * b], 0, 0, 0);
             O[2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(Ah, P, O[2 * b + 1], 0, 0, 0);
             if constexpr (NS == 2) {
                 O[2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(Al, Pl, O[2 * b], 0, 0, 0);
                 O[2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(Ah, Pl, O[2 * b + 1], 0, 0, 0);
             }
+            if (b + AHEAD < NB) vx[b + AHEAD] = v_codes(b + AHEAD);
+            if (b + 1 < NB) v_operands(b + 1);
         }
+        sched_fence();
     }
     // the four waves' sums joined through LDS
     lsum += __shfl_xor(lsum, 16, 64);
@@ -782,7 +812,8 @@ __global__ __launch_bounds__(256, 2) void kv4_split_kernel(Attn a) {
             for (int j = 0; j < 4; j++) o[j] = fmaf(x[j], c, o[j]);
         }
         if (whole) {
-            store_out(a, wk.tok0 + (int)((16 * mt + r) / a.gqa), g * a.gqa + (16 * mt + r) % a.gqa, e, o, l);
+            const uint32_t tk = tok_of(r);
+            store_out(a, wk.tok0 + (int)tk, (g - tk) * a.gqa + 16 * mt + r, e, o, l);
         } else {
             const size_t rec = (((size_t)rec0 * NKV + g) * a.n_mt + mt) * 16 + r;
             *reinterpret_cast<f32x4 *>(a.part + rec * HD + e) = o;
@@ -790,7 +821,7 @@ __global__ __launch_bounds__(256, 2) void kv4_split_kernel(Attn a) {
         }
     }
     }
-    if (blockIdx.x == 0 && w == 0) report_lengths(a);
+    if ((g | slot | mt) == 0 && w == 0) report_lengths(a);
 }
 
 // A sequence divided over slots: out = sum c_i O_i / sum c_i l_i with c_i =
@@ -799,7 +830,7 @@ __global__ __launch_bounds__(256, 2) void kv4_split_kernel(Attn a) {
 // up to 8 NW.
 template <int NW>
 __global__ __launch_bounds__(64 * NW) void kv4_merge_kernel(Attn a, uint32_t rows) {
-    __shared__ float red[NW];
+    __shared__ float2 red[NW];   // a wave's reference and weight sum
     __shared__ __attribute__((aligned(16))) float comb[NW][256];
     const uint32_t r = blockIdx.x % rows, sg = blockIdx.x / rows, g = sg % a.b.nkv, lane = threadIdx.x & 63u, HD = a.b.hd;
     const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -812,8 +843,6 @@ __global__ __launch_bounds__(64 * NW) void kv4_merge_kernel(Attn a, uint32_t row
         return (((size_t)((i0 + c) * 2 + (c == 0 ? head1 : 0u)) * a.b.nkv + g) * a.n_mt + r / 16) * 16 + r % 16;
     };
     float m = REF_NONE, l = 0.0f;
-    for (uint32_t c = lane; c < n; c += 64) m = fmaxf(m, a.ml[rec(c)].x);
-    m = wave_max_f32(m);
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
     const uint32_t e = 4 * lane;
     for (uint32_t c0 = w; c0 < n; c0 += 8 * NW) {
@@ -825,6 +854,13 @@ __global__ __launch_bounds__(64 * NW) void kv4_merge_kernel(Attn a, uint32_t row
             ml[k] = a.ml[at];
             x[k] = *reinterpret_cast<const f32x4 *>(a.part + at * HD + (e < HD ? e : 0u));
         }
+        float mn = m;
+#pragma unroll
+        for (uint32_t k = 0; k < 8; k++) mn = fmaxf(mn, ml[k].x);
+        const float f = __builtin_amdgcn_exp2f(m - mn);
+        l *= f;
+        o = o * f;
+        m = mn;
 #pragma unroll
         for (uint32_t k = 0; k < 8; k++) {
             if (c0 + NW * k >= n) break;
@@ -834,14 +870,21 @@ __global__ __launch_bounds__(64 * NW) void kv4_merge_kernel(Attn a, uint32_t row
             for (int j = 0; j < 4; j++) o[j] = fmaf(x[k][j], c, o[j]);
         }
     }
-    if (lane == 0) red[w] = l;
+    if (lane == 0) red[w] = make_float2(m, l);
     *reinterpret_cast<f32x4 *>(&comb[w][e]) = o;
     __syncthreads();
     if (w != 0 || e >= HD) return;
 #pragma unroll
-    for (uint32_t k = 1; k < NW; k++) {
-        l += red[k];
-        o = o + *reinterpret_cast<const f32x4 *>(&comb[k][e]);
+    for (uint32_t k = 0; k < NW; k++) m = fmaxf(m, red[k].x);
+    l = 0.0f;
+    o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (uint32_t k = 0; k < NW; k++) {
+        const float c = __builtin_amdgcn_exp2f(red[k].x - m);
+        const f32x4 x = *reinterpret_cast<const f32x4 *>(&comb[k][e]);
+        l = fmaf(red[k].y, c, l);
+#pragma unroll
+        for (int j = 0; j < 4; j++) o[j] = fmaf(x[j], c, o[j]);
     }
     store_out(a, wk.tok0 + (int)(r / a.gqa), g * a.gqa + r % a.gqa, e, o, l);
 }
@@ -1535,8 +1578,9 @@ void launch_attn(const Attn &k, const Plan &p, hipStream_t s) {
         else tile(kv4_tile_kernel<HD, SINTER_BF16, tile_waves(false)>);
     }
     if (p.grid) {
-        if (f32) hipLaunchKernelGGL((kv4_split_kernel<HD, 2>), dim3((uint32_t)p.grid), dim3(256), 0, s, k);
-        else hipLaunchKernelGGL((kv4_split_kernel<HD, 1>), dim3((uint32_t)p.grid), dim3(256), 0, s, k);
+        const dim3 grid(k.b.nkv, p.n_slots, p.n_mt);
+        if (f32) hipLaunchKernelGGL((kv4_split_kernel<HD, 2>), grid, dim3(256), 0, s, k);
+        else hipLaunchKernelGGL((kv4_split_kernel<HD, 1>), grid, dim3(256), 0, s, k);
     }
 }
 
@@ -1663,6 +1707,7 @@ int sinter_kv4_attn(const sinter_kv4_batch *b, const sinter_kv4_attn_args *a, vo
     k.n_tile = p.n_tile; k.n_split = p.n_split; k.report = !p.split; k.split_rows = p.split ? SPLIT_ROWS : 0;
     k.page_shift = (uint32_t)__builtin_ctz(b->page_rows);
     k.qscale = a->scale * 1.44269504088896341f;
+    k.gqa_inv = (uint32_t)((((uint64_t)1 << 32) + k.gqa - 1) / k.gqa);
     const hipStream_t s = (hipStream_t)stream;
     if (b->hd == 256) launch_attn<256>(k, p, s);
     else if (b->hd == 128) launch_attn<128>(k, p, s);
