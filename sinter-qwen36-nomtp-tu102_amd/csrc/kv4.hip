@@ -331,32 +331,35 @@ __device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v) {
     return v;
 }
 
+// Of the 64 sequences from `base` on (a lane's: rows, first token, tokens, items
+// c from number lo on), the one that has item `id`, or (by_seq) sequence `id`.
+__device__ __forceinline__ bool pick(Work &w, uint32_t base, uint32_t id, bool by_seq, int len, int t0, int n, uint32_t c,
+                                     uint32_t lo) {
+    const bool mine = c > 0 && (by_seq ? base + (threadIdx.x & 63u) == id : id >= lo && id < lo + c);
+    const uint64_t m = __builtin_amdgcn_ballot_w64(mine);
+    if (m == 0) return false;
+    const int l = __builtin_ctzll(m);
+    w.seq = (int)base + l;
+    w.len = __builtin_amdgcn_readlane(len, l);
+    w.tok0 = __builtin_amdgcn_readlane(t0, l);
+    w.n_new = __builtin_amdgcn_readlane(n, l);
+    w.first = (uint32_t)__builtin_amdgcn_readlane((int)lo, l);
+    w.count = (uint32_t)__builtin_amdgcn_readlane((int)c, l);
+    w.item = by_seq ? 0u : id - w.first;
+    return true;
+}
 // The sequences' items, count(len, n) each, numbered one sequence after the
 // other: item `id`'s sequence, or (by_seq) sequence `id` with its item 0.
 template <class Count>
 __device__ __forceinline__ Work locate(const Attn &a, uint32_t id, bool by_seq, Count count) {
-    const uint32_t lane = threadIdx.x & 63u;
     Work w;
     w.seq = -1;
     uint32_t before = 0;
     for (uint32_t base = 0; base < a.b.n_seq; base += 64) {
         int len, t0, n;
         load_seq(a, base, false, len, t0, n);
-        const uint32_t c = n > 0 ? count(len, n) : 0u;
-        const uint32_t sum = wave_scan_u32(c), lo = before + sum - c;
-        const bool mine = c > 0 && (by_seq ? base + lane == id : id >= lo && id < lo + c);
-        const uint64_t m = __builtin_amdgcn_ballot_w64(mine);
-        if (m != 0) {
-            const int l = __builtin_ctzll(m);
-            w.seq = (int)base + l;
-            w.len = __builtin_amdgcn_readlane(len, l);
-            w.tok0 = __builtin_amdgcn_readlane(t0, l);
-            w.n_new = __builtin_amdgcn_readlane(n, l);
-            w.first = (uint32_t)__builtin_amdgcn_readlane((int)lo, l);
-            w.count = (uint32_t)__builtin_amdgcn_readlane((int)c, l);
-            w.item = by_seq ? 0u : id - w.first;
-            return w;
-        }
+        const uint32_t c = n > 0 ? count(len, n) : 0u, sum = wave_scan_u32(c);
+        if (pick(w, base, id, by_seq, len, t0, n, c, before + sum - c)) return w;
         before += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
     }
     return w;
@@ -392,6 +395,24 @@ __device__ __forceinline__ uint32_t slot_tiles(const Attn &a, uint32_t total) {
 }
 __device__ __forceinline__ Work find_tiles(const Attn &a, uint32_t id, bool by_seq) {
     return locate(a, id, by_seq, [&](int len, int n) { return tiles_of(a, len, n); });
+}
+// All of it at once, where a lane holds every sequence: the total, the tiles a
+// slot, and the work at slot `id`'s first tile or (by_seq) of sequence `id`
+__device__ __forceinline__ Work first_tiles(const Attn &a, uint32_t id, bool by_seq, uint32_t &total, uint32_t &ct) {
+    if (a.b.n_seq <= 64) {
+        int len, t0, n;
+        load_seq(a, 0, false, len, t0, n);
+        const uint32_t c = n > 0 ? tiles_of(a, len, n) : 0u, sum = wave_scan_u32(c);
+        total = (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+        ct = slot_tiles(a, total);
+        Work w;
+        w.seq = -1;
+        pick(w, 0, by_seq ? id : id * ct, by_seq, len, t0, n, c, sum - c);
+        return w;
+    }
+    total = all_tiles(a);
+    ct = slot_tiles(a, total);
+    return find_tiles(a, by_seq ? id : id * ct, by_seq);
 }
 
 // the gated, normalised output of four elements
@@ -483,10 +504,12 @@ __global__ __launch_bounds__(256, 2) void kv4_split_kernel(Attn a) {
     const uint32_t g = blockIdx.x, slot = blockIdx.y, mt = blockIdx.z;
     // (a row's token: rows < 32, gqa <= 32, so the product with ceil(2^32 / gqa) has the quotient)
     auto tok_of = [&](uint32_t r) { return a.gqa == 1 ? 16 * mt + r : __umulhi(16 * mt + r, a.gqa_inv); };
-    const uint32_t total = all_tiles(a), ct = slot_tiles(a, total), x0 = slot * ct, x1 = min(x0 + ct, total);
+    uint32_t total, ct;
+    Work wk = first_tiles(a, slot, false, total, ct);
+    const uint32_t x0 = slot * ct, x1 = min(x0 + ct, total);
     bool again = false;
     for (uint32_t x = x0; x < x1;) {
-    const Work wk = find_tiles(a, x, false);
+    if (x > x0) wk = find_tiles(a, x, false);
     if (wk.seq < 0) break;   // (never: x < total)
     const uint32_t t0 = x - wk.first, t1 = wk.count <= WHOLE ? wk.count : min(x1 - wk.first, wk.count);   // its tiles here
     const bool ours = t0 == 0 || wk.count > WHOLE, whole = t0 == 0 && t1 == wk.count;
@@ -834,9 +857,10 @@ __global__ __launch_bounds__(64 * NW) void kv4_merge_kernel(Attn a, uint32_t row
     __shared__ __attribute__((aligned(16))) float comb[NW][256];
     const uint32_t r = blockIdx.x % rows, sg = blockIdx.x / rows, g = sg % a.b.nkv, lane = threadIdx.x & 63u, HD = a.b.hd;
     const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const Work wk = find_tiles(a, sg / a.b.nkv, true);
+    uint32_t total, ct;
+    const Work wk = first_tiles(a, sg / a.b.nkv, true, total, ct);
     if (wk.seq < 0 || wk.count <= WHOLE || r >= (uint32_t)wk.n_new * a.gqa) return;
-    const uint32_t ct = slot_tiles(a, all_tiles(a)), i0 = wk.first / ct, i1 = (wk.first + wk.count - 1u) / ct;
+    const uint32_t i0 = wk.first / ct, i1 = (wk.first + wk.count - 1u) / ct;
     if (i0 == i1) return;
     const uint32_t n = i1 - i0 + 1u, head1 = wk.first > i0 * ct ? 1u : 0u;   // (its first segment: the slot's own first, or its last)
     auto rec = [&](uint32_t c) {
@@ -1516,9 +1540,10 @@ int check_attn(const sinter_kv4_batch *b, const sinter_kv4_attn_args *a) {
 constexpr uint32_t tile_waves(bool f32) { return f32 ? 4 : 8; }
 
 // The launches of a batch.  kv4_split_kernel: row tiles a sequence, and slots,
-// as many as run at once (two workgroups a CU).  kv4_tile_kernel: row tiles (at most one
+// as many as run at once.  kv4_tile_kernel: row tiles (at most one
 // partly filled one a sequence) and chunks of the cache rows a tile sees.
-constexpr uint32_t SLOTS = 512;
+// (two workgroups a CU by their LDS with heads of 256, by registers three and four with 128 and 64)
+uint32_t slots_at_once(uint32_t hd) { return hd == 256 ? 512 : hd == 128 ? 768 : 1024; }
 struct Plan {
     uint32_t n_mt = 0, n_slots = 0, n_tile = 0, n_split = 1;
     bool split = false, merge = false, join = false;
@@ -1538,7 +1563,7 @@ Plan make_plan(const sinter_kv4_batch &b, const sinter_kv4_attn_args &a) {
         p.merge = a.max_kv > WHOLE * TILE;
         const uint64_t per = (uint64_t)b.nkv * p.n_mt;
         const uint64_t most = (uint64_t)b.n_seq * std::max<uint64_t>(1, (a.max_kv + CT_MIN * TILE - 1) / (CT_MIN * TILE));
-        p.n_slots = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(1, SLOTS / per), most);
+        p.n_slots = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(1, slots_at_once(b.hd) / per), most);
         p.grid = (uint64_t)p.n_slots * b.nkv * p.n_mt;
         p.recs = p.merge ? (size_t)p.grid * 32 : 0;
     }
