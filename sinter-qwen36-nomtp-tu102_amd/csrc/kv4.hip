@@ -31,6 +31,7 @@ namespace {
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ f16x2 pair_of(uint32_t w) { return __builtin_bit_cast(f16x2, w); }
 typedef uint16_t __attribute__((may_alias)) u16a;   // (written as halves, read as wider words)
@@ -48,7 +49,10 @@ __device__ __forceinline__ float4 cvt4(u32x2 u, uint32_t type) {
     return make_float4(h2f((uint16_t)u.x), h2f((uint16_t)(u.x >> 16)), h2f((uint16_t)u.y), h2f((uint16_t)(u.y >> 16)));
 }
 __device__ __forceinline__ uint32_t pack2(float a, float b, uint32_t type) {
-    if (type == SINTER_BF16) return (uint32_t)f2bf(a) | ((uint32_t)f2bf(b) << 16);
+    if (type == SINTER_BF16) {   // (one instruction, to nearest even)
+        const bf16x2 v = {(__bf16)a, (__bf16)b};
+        return __builtin_bit_cast(uint32_t, v);
+    }
     return (uint32_t)f2h(a) | ((uint32_t)f2h(b) << 16);
 }
 // four elements at element `e` (a multiple of 4) of a buffer of `type`
@@ -64,6 +68,20 @@ __device__ __forceinline__ void store4(void *p, int64_t e, uint32_t type, float4
     const u32x2 u = {pack2(v.x, v.y, type), pack2(v.z, v.w, type)};
     *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(p) + e) = u;
 }
+
+// Four elements as they lie: loads are issued together, conversions come later
+template <uint32_t T>
+struct Raw4 {
+    typename std::conditional<T == SINTER_F32, f32x4, u32x2>::type v;
+    __device__ __forceinline__ void load(const void *p, int64_t e) {
+        if constexpr (T == SINTER_F32) v = *reinterpret_cast<const f32x4 *>(static_cast<const float *>(p) + e);
+        else v = *reinterpret_cast<const u32x2 *>(static_cast<const uint16_t *>(p) + e);
+    }
+    __device__ __forceinline__ float4 get() const {
+        if constexpr (T == SINTER_F32) return make_float4(v.x, v.y, v.z, v.w);
+        else return cvt4(v, T);
+    }
+};
 
 // ------------------------------------------------------------------ the batch
 
@@ -82,22 +100,62 @@ __device__ __forceinline__ int seq_of(const sinter_kv4_batch &b, uint32_t t) {
     return -1;
 }
 
-// the position of token t, or -1 where it has none (behind the last sequence,
-// or before row 0 of its own)
-__device__ __forceinline__ int token_pos(const sinter_kv4_batch &b, uint32_t t, int &seq) {
-    seq = seq_of(b, t);
-    if (seq < 0) return -1;
-    return max(b.kv_len[seq] - (b.tok_start[seq + 1] - (int)t), -1);
+// Where tokens t0 .. t0 + n - 1 (n <= 64) stand: lane k gets token t0 + k's
+// sequence and position (-1 where it has none: behind the last sequence, or
+// before row 0 of its own).  Sixty-four sequences' bounds are loaded at once
+// and the tokens found among them without further loads.
+__device__ __forceinline__ void token_places(const sinter_kv4_batch &b, uint32_t t0, uint32_t n, int &seq, int &pos) {
+    const uint32_t lane = threadIdx.x & 63u;
+    seq = pos = -1;
+    uint32_t k = 0;
+    for (uint32_t base = 0; base < b.n_seq && k < n; base += 64) {
+        const uint32_t i = min(base + lane, b.n_seq - 1u);
+        const int start = b.tok_start[i], stop = b.tok_start[i + 1], len = b.kv_len[i];
+        for (; k < n; k++) {
+            const int t = (int)(t0 + k);
+            const uint64_t m = __builtin_amdgcn_ballot_w64(base + lane < b.n_seq && stop > t);
+            if (m == 0) break;   // (in the next sequences, or behind all)
+            const int l = __builtin_ctzll(m);
+            if (__builtin_amdgcn_readlane(start, l) > t) continue;
+            const int p = __builtin_amdgcn_readlane(len, l) - (__builtin_amdgcn_readlane(stop, l) - t);
+            if (lane == k && p >= 0) {
+                seq = (int)base + l;
+                pos = p;
+            }
+        }
+    }
 }
 
-// the page that row `pos` of sequence `seq` lies in, or -1 (and the error
-// raised) where the table has none
-__device__ __forceinline__ int page_of(const sinter_kv4_batch &b, int seq, int pos) {
-    const uint32_t e = (uint32_t)pos / b.page_rows;
-    const int page = e < b.max_pages ? b.pages[(size_t)seq * b.max_pages + e] : -1;
-    if ((uint32_t)page < b.n_pages) return page;
-    if ((threadIdx.x & 63u) == 0) raise_error(g_kv4_err, SINTER_E_BAD_SHAPE, (unsigned)seq);
-    return -1;
+// Tokens a workgroup of append and read takes at most: their places are found
+// together (reading 20 sequences, F32: 4 tokens 68 us, 8 71 us, 16 83 us, one 98)
+constexpr uint32_t TOKS = 4;
+
+// The cache rows of tokens t0 .. t0 + n - 1 (n <= TOKS) for a workgroup: byte
+// offset of their page (or -1: none, with the error raised where the table has
+// no page for a row) and row in it.
+struct TokRows {
+    uint64_t page[TOKS];
+    uint32_t row[TOKS];
+};
+__device__ __forceinline__ void token_rows(const sinter_kv4_batch &b, uint32_t t0, uint32_t n, size_t page_bytes, TokRows &rows) {
+    if (threadIdx.x < 64) {
+        int seq, pos;
+        token_places(b, t0, n, seq, pos);
+        if (threadIdx.x < n) {
+            int page = -1;
+            if (pos >= 0) {
+                const uint32_t e = (uint32_t)pos / b.page_rows;
+                page = e < b.max_pages ? b.pages[(size_t)seq * b.max_pages + e] : -1;
+                if ((uint32_t)page >= b.n_pages) {
+                    raise_error(g_kv4_err, SINTER_E_BAD_SHAPE, (unsigned)seq);
+                    page = -1;
+                }
+            }
+            rows.page[threadIdx.x] = page < 0 ? ~0ull : (uint64_t)(uint32_t)page * page_bytes;
+            rows.row[threadIdx.x] = page < 0 ? 0u : (uint32_t)pos & (b.page_rows - 1u);
+        }
+    }
+    __syncthreads();
 }
 
 // ------------------------------------------------------------------ prep
@@ -107,59 +165,102 @@ struct Prep {
     sinter_heads q, q_out, k, k_out;
     const float *q_norm, *k_norm;
     double rate;   // log2(base) / (rope_dims / 2)
-    uint32_t nq, half, type, heads;
-    float eps;
+    uint32_t nq, nk, half;
+    float eps, inv_hd;
 };
 
 // y = x / sqrt(mean(x^2) + eps) * w, then the pairs (i, i + half) turned by
 // pos * base^(-i / half).  The angle is held in turns in fp64 (at position
 // 131072 an fp32 angle is off by thousandths of a radian), once a token and
-// workgroup.  A head is hd / 4 lanes of four elements.  blockIdx.y: a
-// workgroup's share of the heads.
+// workgroup.  A head is hd / 8 lanes of two times four elements: those of a
+// pair in one lane, so that nothing moves between lanes but the sum of
+// squares.  A wave takes `per` heads of one kind at a time; blockIdx.y: a
+// workgroup's share of them.
+// The heads' loads are issued before the angles, whose fp64 the time is for
+// few tokens (one token of 24 + 4 heads of 256: 4 us of the kernel, all
+// latency).  Of many the rows' traffic: 2557 tokens of 28 heads of 256, bf16,
+// 73 MB in and out in 16 us, 4.6 TB/s where a copy reaches 5.2 (with a pair's
+// halves in two lanes and four elements a lane 26 us, bound by instructions;
+// the weights read again for every head 8 % more).
+template <uint32_t T>
 __global__ __launch_bounds__(256) void kv4_prep_kernel(Prep a) {
     __shared__ float2 turn[128];
     const uint32_t t = blockIdx.x, lane = threadIdx.x & 63u;
-    int seq;
-    const int pos = token_pos(a.b, t, seq);
+    const uint32_t hd = a.b.hd, lph = hd / 8, l = lane % lph, hl = lane / lph, per = 64 / lph;
+    const uint32_t quarter = a.half / 4, step = gridDim.y * 4;
+    const uint32_t first = blockIdx.y * 4 + (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const uint32_t uq = (a.nq + per - 1) / per, units = uq + (a.nk + per - 1) / per;
+    const bool in = l < quarter;   // (its eight elements are four pairs)
+    const uint32_t e0 = in ? 4 * l : 8 * l, e1 = in ? e0 + a.half : e0 + 4;
+    struct X { Raw4<T> lo, hi; };
+    auto fetch = [&](uint32_t u) {
+        X x = {};
+        const bool isq = u < uq;
+        const uint32_t h = (isq ? u : u - uq) * per + hl;
+        const sinter_heads &p = isq ? a.q : a.k;
+        if (u < units && h < (isq ? a.nq : a.nk)) {
+            const int64_t at = (int64_t)t * p.ld + (int64_t)h * p.hs;
+            x.lo.load(p.p, at + e0);
+            x.hi.load(p.p, at + e1);
+        }
+        return x;
+    };
+    // (a token that is nobody's has its row in the arrays too)
+    X x0 = fetch(first), x1 = fetch(first + step);
+    float4 w[2][2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const float *n = k ? a.k_norm : a.q_norm;
+        w[k][0] = w[k][1] = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+        if (n) {
+            w[k][0] = *reinterpret_cast<const float4 *>(n + e0);
+            w[k][1] = *reinterpret_cast<const float4 *>(n + e1);
+        }
+    }
+    int seq, pos;
+    token_places(a.b, t, 1, seq, pos);
+    pos = __builtin_amdgcn_readfirstlane(pos);
     if (pos < 0) return;   // (uniform)
     if (threadIdx.x < a.half) {
         const double f = exp2(-(double)threadIdx.x * a.rate) * 0.15915494309189533577;   // 1 / (2 pi)
-        const double x = (double)pos * f, fr = x - rint(x);
+        const double y = (double)pos * f, fr = y - rint(y);
         double s, c;
         sincospi(2.0 * fr, &s, &c);
         turn[threadIdx.x] = make_float2((float)c, (float)s);
     }
     __syncthreads();
-    const uint32_t hd = a.b.hd, lph = hd / 4, l = lane % lph, wave = threadIdx.x >> 6, per = 64 / lph;
-    const uint32_t quarter = a.half / 4;
-    for (uint32_t h0 = (blockIdx.y * 4 + wave) * per; h0 < a.heads; h0 += gridDim.y * 4 * per) {
-        const uint32_t h = h0 + lane / lph;
-        const bool live = h < a.heads;
-        const bool isq = h < a.nq;
-        const uint32_t hh = live ? (isq ? h : h - a.nq) : 0u;
-        const sinter_heads &src = !live || isq ? a.q : a.k, &dst = !live || isq ? a.q_out : a.k_out;
-        const float *w = !live || isq ? a.q_norm : a.k_norm;
-        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (live) x = load4(src.p, (int64_t)t * src.ld + (int64_t)hh * src.hs + 4 * l, a.type);
-        float ss = lanes_sum_f32(x.x * x.x + x.y * x.y + (x.z * x.z + x.w * x.w), lph);
-        const float r = 1.0f / sqrtf(ss / (float)hd + a.eps);
-        float y[4] = {x.x * r, x.y * r, x.z * r, x.w * r};
-        if (w) {
-            const float4 wt = reinterpret_cast<const float4 *>(w)[l];
-            y[0] *= wt.x; y[1] *= wt.y; y[2] *= wt.z; y[3] *= wt.w;
-        }
-        const bool lo = l < quarter, in = l < 2 * quarter;
-        const int partner = (int)(lane + (lo ? quarter : in ? 0u - quarter : 0u));
+    float2 cs[4];
 #pragma unroll
-        for (uint32_t c = 0; c < 4; c++) {
-            const float o = __shfl(y[c], partner, 64);
-            if (in) {
-                const float2 cs = turn[4 * (lo ? l : l - quarter) + c];
-                y[c] = y[c] * cs.x + (lo ? -o : o) * cs.y;
+    for (uint32_t c = 0; c < 4; c++) cs[c] = in ? turn[4 * l + c] : make_float2(1.0f, 0.0f);
+    for (uint32_t u = first; u < units; u += step) {
+        const float4 lo = x0.lo.get(), hi = x0.hi.get();
+        x0 = x1;
+        x1 = fetch(u + 2 * step);
+        const float ss = lanes_sum_f32((lo.x * lo.x + lo.y * lo.y + (lo.z * lo.z + lo.w * lo.w)) + (hi.x * hi.x + hi.y * hi.y + (hi.z * hi.z + hi.w * hi.w)), lph);
+        const float r = 1.0f / sqrtf(ss * a.inv_hd + a.eps);
+        float y[8] = {lo.x * r, lo.y * r, lo.z * r, lo.w * r, hi.x * r, hi.y * r, hi.z * r, hi.w * r};
+        const bool isq = u < uq;
+        auto weigh = [&](const float4 &w0, const float4 &w1) {
+            y[0] *= w0.x; y[1] *= w0.y; y[2] *= w0.z; y[3] *= w0.w;
+            y[4] *= w1.x; y[5] *= w1.y; y[6] *= w1.z; y[7] *= w1.w;
+        };
+        if (isq) weigh(w[0][0], w[0][1]);
+        else weigh(w[1][0], w[1][1]);
+        if (in) {
+#pragma unroll
+            for (uint32_t c = 0; c < 4; c++) {
+                const float p = y[c], o = y[c + 4];
+                y[c] = p * cs[c].x - o * cs[c].y;
+                y[c + 4] = o * cs[c].x + p * cs[c].y;
             }
         }
-        if (live)
-            store4(dst.p, (int64_t)t * dst.ld + (int64_t)hh * dst.hs + 4 * l, a.type, make_float4(y[0], y[1], y[2], y[3]));
+        const uint32_t h = (isq ? u : u - uq) * per + hl;
+        if (h < (isq ? a.nq : a.nk)) {
+            const sinter_heads &p = isq ? a.q_out : a.k_out;
+            const int64_t at = (int64_t)t * p.ld + (int64_t)h * p.hs;
+            store4(p.p, at + e0, T, make_float4(y[0], y[1], y[2], y[3]));
+            store4(p.p, at + e1, T, make_float4(y[4], y[5], y[6], y[7]));
+        }
     }
 }
 
@@ -168,98 +269,156 @@ __global__ __launch_bounds__(256) void kv4_prep_kernel(Prep a) {
 struct Rows {
     sinter_kv4_batch b;
     sinter_heads k, v;
-    uint32_t type, per;   // per: workgroups a token
+    uint32_t toks, parts;   // tokens a workgroup; workgroups that share them
 };
 
-// Eight lanes quantise one block of 32, four elements each: m = the first
+// Four lanes quantise one block of 32, eight elements each: m = the first
 // element of the largest magnitude (saturated at the f16 maximum), d = m / -8,
 // code = min(15, trunc(x / d + 8.5)) by the product with 1 / d, in fp32 with
 // every product and sum rounded (ggml's Q4_0 reference quantiser).  A block
 // whose f16 scale is zero has every code 8; one with a NaN has a NaN scale.
+// A workgroup takes several tokens, whose places are found together, and four
+// blocks' loads at a time.  Bound by instructions (about 200 for a wave's 16
+// blocks, ten of the time's microseconds) before the rows' traffic: 32 MB of
+// bf16 rows of 8 heads of 128 into 9 MB of pages in 15 us, 2.7 TB/s (eight lanes a block, each with its own division and search: 20 us; a
+// workgroup a token, one block's loads at a time, 24 us).
+template <uint32_t T>
 __global__ __launch_bounds__(256) void kv4_append_kernel(Rows a) {
-    const uint32_t t = blockIdx.x / a.per, lane = threadIdx.x & 63u;
-    const uint32_t nb = a.b.hd / 32, nblk = a.b.nkv * nb;
-    int seq;
-    const int pos = token_pos(a.b, t, seq);
-    if (pos < 0) return;
-    const int page = page_of(a.b, seq, pos);
-    if (page < 0) return;
-    const uint32_t i = (blockIdx.x % a.per) * 32u + threadIdx.x / 8u;   // K's blocks, then V's
-    if (i >= 2 * nblk) return;                                           // (whole groups of eight lanes)
-    const bool isv = i >= nblk;
-    const uint32_t j = isv ? i - nblk : i, g = j / nb, bl = j % nb, l8 = lane & 7u;
-    const sinter_heads &src = isv ? a.v : a.k;
-    const float4 x4 = load4(src.p, (int64_t)t * src.ld + (int64_t)g * src.hs + 32 * bl + 4 * l8, a.type);
-    float x[4] = {x4.x, x4.y, x4.z, x4.w};
-    float am = 0.0f;
-    bool nan = false;
+    __shared__ TokRows tok;
+    const uint32_t nb = a.b.hd / 32, nblk = a.b.nkv * nb, rows = a.b.page_rows, hb = a.b.hd / 2;
+    const size_t head_bytes = (size_t)rows * (hb + hb / 8);
+    const uint32_t grp = blockIdx.x / a.parts, part = blockIdx.x % a.parts, t0 = grp * a.toks, n = min(a.toks, a.b.n_tok - t0);
+    token_rows(a.b, t0, n, head_bytes * a.b.nkv, tok);
+    // block j of a token (K's, then V's) stays with its four lanes, token after token
+    const uint32_t l4 = threadIdx.x & 3u, wide = min(2 * nblk, 64u), step = 64u / wide, k0 = threadIdx.x / 4u / wide;
+    if (k0 >= step) return;
+    for (uint32_t j0 = part * wide + threadIdx.x / 4u % wide; j0 < 2 * nblk; j0 += wide * a.parts) {
+        const bool isv = j0 >= nblk;
+        const uint32_t j = isv ? j0 - nblk : j0, g = j / nb, bl = j % nb;
+        const int64_t ld = isv ? a.v.ld : a.k.ld, at0 = (int64_t)g * (isv ? a.v.hs : a.k.hs) + 32 * bl + 8 * l4;
+        const void *src = isv ? a.v.p : a.k.p;
+        unsigned char *plane = static_cast<unsigned char *>(isv ? a.b.vc : a.b.kc) + g * head_bytes;
+        for (uint32_t kb = k0; kb < n; kb += 4 * step) {
+            Raw4<T> in[4][2];
 #pragma unroll
-    for (int c = 0; c < 4; c++) {
-        nan |= x[c] != x[c];
-        x[c] = fminf(fmaxf(x[c], -F16_MAX), F16_MAX);
-        am = fmaxf(am, fabsf(x[c]));
+            for (uint32_t u = 0; u < 4; u++) {
+                const int64_t at = (int64_t)(t0 + min(kb + u * step, n - 1u)) * ld + at0;
+                in[u][0].load(src, at);
+                in[u][1].load(src, at + 4);
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < 4; u++) {
+                const uint32_t k = kb + u * step;
+                if (k >= n || tok.page[k] == ~0ull) continue;   // (the same for a block's four lanes)
+                const float4 f0 = in[u][0].get(), f1 = in[u][1].get();
+                float x[8] = {f0.x, f0.y, f0.z, f0.w, f1.x, f1.y, f1.z, f1.w};
+                int nan = 0;
+#pragma unroll
+                for (int c = 0; c < 8; c += 2) nan |= __builtin_isunordered(x[c], x[c + 1]);
+                float hi = -F16_MAX, lo = F16_MAX;   // (a NaN leaves them)
+#pragma unroll
+                for (int c = 0; c < 8; c++) {
+                    x[c] = __builtin_amdgcn_fmed3f(x[c], -F16_MAX, F16_MAX);
+                    hi = fmaxf(hi, x[c]);
+                    lo = fminf(lo, x[c]);
+                }
+                hi = fmaxf(hi, dpp_f<DPP_XOR1>(hi));
+                lo = fminf(lo, dpp_f<DPP_XOR1>(lo));
+                nan |= dpp_i<DPP_XOR1>(nan);
+                hi = fmaxf(hi, dpp_f<DPP_XOR2>(hi));
+                lo = fminf(lo, dpp_f<DPP_XOR2>(lo));
+                nan |= dpp_i<DPP_XOR2>(nan);
+                bool pos = hi > -lo;
+                if (__builtin_amdgcn_ballot_w64(hi == -lo) != 0) {   // both signs have the largest magnitude: which comes first
+                    int at = 64;
+#pragma unroll
+                    for (int c = 7; c >= 0; c--)
+                        if (fabsf(x[c]) == hi) at = 2 * (int)(8 * l4 + c) + (x[c] > 0.0f ? 1 : 0);
+                    at = min(at, dpp_i<DPP_XOR1>(at));
+                    at = min(at, dpp_i<DPP_XOR2>(at));
+                    if (hi == -lo) pos = at & 1;
+                }
+                const float d = (pos ? hi : lo) / -8.0f;
+                uint16_t dh = f2h(d);
+                const bool zero = (dh & 0x7fffu) == 0;
+                if (zero) dh = 0;
+                if (nan) dh = 0x7e00u;
+                const float inv = zero ? 0.0f : 1.0f / d;
+                uint32_t q[2];
+#pragma unroll
+                for (int p = 0; p < 2; p++) {
+                    q[p] = 0;
+#pragma unroll
+                    for (int c = 0; c < 4; c++) q[p] |= (uint32_t)(int)(x[4 * p + c] * inv + 8.5f) << (8 * c);
+                    q[p] -= (q[p] >> 4) & 0x01010101u;   // (16 is 15)
+                    if (nan) q[p] = 0x08080808u;
+                    // lane l4 < 2 joins lane l4 + 2's codes (elements 16 further) above its own
+                    q[p] |= (uint32_t)dpp_i<DPP_XOR2>((int)q[p]) << 4;
+                }
+                unsigned char *head = plane + tok.page[k];
+                const uint32_t row = tok.row[k];
+                if (l4 < 2) *reinterpret_cast<u32x2 *>(head + (size_t)row * hb + 16 * bl + 8 * l4) = u32x2{q[0], q[1]};
+                if (l4 == 0) *reinterpret_cast<uint16_t *>(head + (size_t)rows * hb + (size_t)row * (hb / 8) + 2 * bl) = dh;
+            }
+        }
     }
-    am = fmaxf(am, dpp_f<DPP_XOR1>(am));
-    am = fmaxf(am, dpp_f<DPP_XOR2>(am));
-    am = fmaxf(am, dpp_f<DPP_HALF_MIRROR>(am));
-    // the first element of that magnitude: its place and sign in one integer
-    int at = 64 + (nan ? -128 : 0);
-#pragma unroll
-    for (int c = 3; c >= 0; c--)
-        if (fabsf(x[c]) == am && !nan) at = 2 * (int)(4 * l8 + c) + (x[c] > 0.0f ? 1 : 0);
-    at = min(at, dpp_i<DPP_XOR1>(at));
-    at = min(at, dpp_i<DPP_XOR2>(at));
-    at = min(at, dpp_i<DPP_HALF_MIRROR>(at));
-    const float d = (at & 1 ? am : -am) / -8.0f;
-    uint16_t dh = f2h(d);
-    const bool zero = (dh & 0x7fffu) == 0;
-    if (zero) dh = 0;
-    if (at < 0) dh = 0x7e00u;
-    const float inv = zero ? 0.0f : 1.0f / d;
-    uint32_t q = 0;
-#pragma unroll
-    for (int c = 0; c < 4; c++) q |= (uint32_t)min(15, (int)(x[c] * inv + 8.5f)) << (8 * c);
-    if (at < 0) q = 0x08080808u;
-    // lane l8 < 4 joins lane l8 + 4's codes (elements 16 further) above its own
-    const uint32_t hi = (uint32_t)dpp_i<0x1B>(dpp_i<DPP_HALF_MIRROR>((int)q));   // (quad_perm [3,2,1,0])
-    const uint32_t rows = a.b.page_rows, hb = a.b.hd / 2, row = (uint32_t)pos & (rows - 1u);
-    unsigned char *head = static_cast<unsigned char *>(isv ? a.b.vc : a.b.kc) +
-                          ((size_t)(uint32_t)page * a.b.nkv + g) * ((size_t)rows * (hb + hb / 8));
-    if (l8 < 4) *reinterpret_cast<uint32_t *>(head + (size_t)row * hb + 16 * bl + 4 * l8) = q | (hi << 4);
-    if (l8 == 0) *reinterpret_cast<uint16_t *>(head + (size_t)rows * hb + (size_t)row * (hb / 8) + 2 * bl) = dh;
 }
 
 // ------------------------------------------------------------------ read
 
-// A thread gives back the 16 elements of eight code bytes (half a block).
+// A thread gives back EL consecutive elements, 16 bytes of F32 (EL = 4) or of a
+// 16-bit type (8): the low or the high four bits of EL code bytes, so that a
+// wave's stores are consecutive (the two halves of a block read its bytes
+// twice, the second time from the cache); four of them in flight.  Bound by the
+// stores: 47 MB of pages and 240 MB of F32 rows in 55 us, 5.2 TB/s, a copy's
+// rate (a workgroup a token, the two halves' stores apart: 85 us).
+template <uint32_t T>
 __global__ __launch_bounds__(256) void kv4_read_kernel(Rows a) {
-    const uint32_t t = blockIdx.x / a.per;
-    const uint32_t nb = a.b.hd / 32, nun = a.b.nkv * nb * 2;
-    int seq;
-    const int pos = token_pos(a.b, t, seq);
-    if (pos < 0) return;
-    const int page = page_of(a.b, seq, pos);
-    if (page < 0) return;
-    const uint32_t i = (blockIdx.x % a.per) * 256u + threadIdx.x;
-    if (i >= 2 * nun) return;
-    const bool isv = i >= nun;
-    const sinter_heads &dst = isv ? a.v : a.k;
-    if (!dst.p) return;
-    const uint32_t j = isv ? i - nun : i, g = j / (2 * nb), bl = (j / 2) % nb, hf = j & 1u;
-    const uint32_t rows = a.b.page_rows, hb = a.b.hd / 2, row = (uint32_t)pos & (rows - 1u);
-    const unsigned char *head = static_cast<const unsigned char *>(isv ? a.b.vc : a.b.kc) +
-                                ((size_t)(uint32_t)page * a.b.nkv + g) * ((size_t)rows * (hb + hb / 8));
-    const u32x2 w = *reinterpret_cast<const u32x2 *>(head + (size_t)row * hb + 16 * bl + 8 * hf);
-    const float d = h2f(*reinterpret_cast<const uint16_t *>(head + (size_t)rows * hb + (size_t)row * (hb / 8) + 2 * bl));
-    const int64_t e = (int64_t)t * dst.ld + (int64_t)g * dst.hs + 32 * bl + 8 * hf;
+    constexpr uint32_t EL = T == SINTER_F32 ? 4 : 8;
+    __shared__ TokRows tok;
+    const uint32_t rows = a.b.page_rows, hb = a.b.hd / 2, uh = a.b.hd / EL, half = a.b.nkv * uh;   // units a head, a token's K or V
+    const size_t head_bytes = (size_t)rows * (hb + hb / 8);
+    const uint32_t grp = blockIdx.x / a.parts, part = blockIdx.x % a.parts, t0 = grp * a.toks, n = min(a.toks, a.b.n_tok - t0);
+    token_rows(a.b, t0, n, head_bytes * a.b.nkv, tok);
+    // unit j of a token (K's, then V's) stays with its thread, token after token
+    const uint32_t upt = (a.k.p && a.v.p ? 2u : 1u) * half, wide = min(upt, 256u), step = 256u / wide, k0 = threadIdx.x / wide;
+    if (k0 >= step) return;
+    for (uint32_t j0 = part * wide + threadIdx.x % wide; j0 < upt; j0 += wide * a.parts) {
+        const bool isv = j0 >= half || !a.k.p;
+        const uint32_t j = j0 >= half ? j0 - half : j0, g = j / uh, e = EL * (j % uh), sh = e & 16u ? 4u : 0u;
+        const unsigned char *codes = static_cast<const unsigned char *>(isv ? a.b.vc : a.b.kc) + g * head_bytes + 16 * (e / 32) + e % 16;
+        const unsigned char *scales = codes - 16 * (e / 32) - e % 16 + (size_t)rows * hb + 2 * (e / 32);
+        const sinter_heads &dst = isv ? a.v : a.k;
+        for (uint32_t kb = k0; kb < n; kb += 4 * step) {
+            u32x2 w[4];
+            uint16_t sc[4];
 #pragma unroll
-    for (uint32_t s = 0; s < 2; s++)
+            for (uint32_t u = 0; u < 4; u++) {
+                const uint32_t k = min(kb + u * step, n - 1u), row = tok.row[k];
+                const uint64_t page = tok.page[k] == ~0ull ? 0 : tok.page[k];   // (a row without a page: page 0's, not kept)
+                const unsigned char *c = codes + page + (size_t)row * hb;
+                if constexpr (EL == 8) w[u] = *reinterpret_cast<const u32x2 *>(c);
+                else w[u].x = *reinterpret_cast<const uint32_t *>(c);
+                sc[u] = *reinterpret_cast<const uint16_t *>(scales + page + (size_t)row * (hb / 8));
+            }
 #pragma unroll
-        for (uint32_t c = 0; c < 2; c++) {
-            const uint32_t u = (c ? w.y : w.x) >> (4 * s);
-            auto val = [&](uint32_t k) { return (float)((int)((u >> (8 * k)) & 15u) - 8) * d; };
-            store4(dst.p, e + 16 * s + 4 * c, a.type, make_float4(val(0), val(1), val(2), val(3)));
+            for (uint32_t u = 0; u < 4; u++) {
+                const uint32_t k = kb + u * step;
+                if (k >= n || tok.page[k] == ~0ull) continue;
+                const int64_t to = (int64_t)(t0 + k) * dst.ld + (int64_t)g * dst.hs + e;
+                const float d = h2f(sc[u]);
+                float v[EL];
+#pragma unroll
+                for (uint32_t i = 0; i < EL; i++) v[i] = (float)((int)(((i < 4 ? w[u].x : w[u].y) >> (8 * (i & 3u) + sh)) & 15u) - 8) * d;
+                if constexpr (EL == 4) {
+                    *reinterpret_cast<float4 *>(static_cast<float *>(dst.p) + to) = make_float4(v[0], v[1], v[2], v[3]);
+                } else {
+                    const u32x4 o = {pack2(v[0], v[1], T), pack2(v[2], v[3], T), pack2(v[4], v[5], T), pack2(v[6], v[7], T)};
+                    *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(dst.p) + to) = o;
+                }
+            }
         }
+    }
 }
 
 // ------------------------------------------------------------------ attention
@@ -1542,6 +1701,25 @@ constexpr uint32_t tile_waves(bool f32) { return f32 ? 4 : 8; }
 // The launches of a batch.  kv4_split_kernel: row tiles a sequence, and slots,
 // as many as run at once.  kv4_tile_kernel: row tiles (at most one
 // partly filled one a sequence) and chunks of the cache rows a tile sees.
+// f(the type as a constant)
+template <class F>
+void by_type(uint32_t type, F f) {
+    if (type == SINTER_F32) f(std::integral_constant<uint32_t, SINTER_F32>());
+    else if (type == SINTER_F16) f(std::integral_constant<uint32_t, SINTER_F16>());
+    else f(std::integral_constant<uint32_t, SINTER_BF16>());
+}
+
+// Tokens a workgroup of append or read, and workgroups that share them, for
+// `units` of a token of which a workgroup takes `wide` at a time: few tokens
+// spread over many workgroups, many are taken together while that leaves
+// 2048 workgroups.
+uint64_t rows_grid(Rows &r, uint32_t units, uint32_t wide) {
+    r.toks = std::min(TOKS, std::max(1u, r.b.n_tok / 2048u));
+    const uint32_t groups = (r.b.n_tok + r.toks - 1) / r.toks;
+    r.parts = std::min((units + wide - 1) / wide, std::max(1u, 2048u / groups));
+    return (uint64_t)groups * r.parts;
+}
+
 // (two workgroups a CU by their LDS with heads of 256, by registers three and four with 128 and 64)
 uint32_t slots_at_once(uint32_t hd) { return hd == 256 ? 512 : hd == 128 ? 768 : 1024; }
 struct Plan {
@@ -1654,12 +1832,14 @@ int sinter_kv4_prep(const sinter_kv4_batch *b, const sinter_kv4_prep_args *a, vo
     p.b = *b;
     p.q = a->q; p.q_out = a->q_out; p.k = a->k; p.k_out = a->k_out;
     p.q_norm = a->q_norm; p.k_norm = a->k_norm;
-    p.nq = nq; p.heads = nq + nk; p.half = a->rope_dims / 2; p.type = a->type; p.eps = a->eps;
+    p.nq = nq; p.nk = nk; p.half = a->rope_dims / 2; p.eps = a->eps; p.inv_hd = 1.0f / (float)b->hd;   // (a power of two)
     p.rate = p.half ? std::log2((double)a->rope_base) / p.half : 0.0;
-    // few tokens: a wave a head group; many: a workgroup a token
-    const uint32_t per = 4 * (256 / b->hd), need = (p.heads + per - 1) / per;
-    const uint32_t y = b->n_tok >= 1024 ? 1u : need;
-    hipLaunchKernelGGL(kv4_prep_kernel, dim3(b->n_tok, y), dim3(256), 0, (hipStream_t)stream, p);
+    // few tokens: a wave takes one group of heads; many: a workgroup a token
+    const uint32_t per = 512 / b->hd, need = ((nq + per - 1) / per + (nk + per - 1) / per + 3) / 4;
+    const dim3 grid(b->n_tok, b->n_tok >= 1024 ? 1u : need);
+    by_type(a->type, [&](auto t) {
+        hipLaunchKernelGGL(kv4_prep_kernel<decltype(t)::value>, grid, dim3(256), 0, (hipStream_t)stream, p);
+    });
     return hip_ok(hipGetLastError(), "kv4_prep: launch") ? SINTER_OK : SINTER_ERR_HIP;
 }
 
@@ -1673,11 +1853,12 @@ int sinter_kv4_append(const sinter_kv4_batch *b, const sinter_heads *k, const si
     if ((why = check_heads(*k, b->n_tok, b->nkv, b->hd, type)) || (why = check_heads(*v, b->n_tok, b->nkv, b->hd, type)))
         return set_error(SINTER_ERR_ARG, "kv4_append: %s", why);
     Rows r;
-    r.b = *b; r.k = *k; r.v = *v; r.type = (uint32_t)type;
-    r.per = (2 * b->nkv * (b->hd / 32) + 31) / 32;
-    const uint64_t grid = (uint64_t)b->n_tok * r.per;
+    r.b = *b; r.k = *k; r.v = *v;
+    const uint64_t grid = rows_grid(r, 2 * b->nkv * (b->hd / 32), 64);
     if (grid > (uint64_t)INT32_MAX) return set_error(SINTER_ERR_ARG, "kv4_append: too many tokens");
-    hipLaunchKernelGGL(kv4_append_kernel, dim3((uint32_t)grid), dim3(256), 0, (hipStream_t)stream, r);
+    by_type((uint32_t)type, [&](auto t) {
+        hipLaunchKernelGGL(kv4_append_kernel<decltype(t)::value>, dim3((uint32_t)grid), dim3(256), 0, (hipStream_t)stream, r);
+    });
     return hip_ok(hipGetLastError(), "kv4_append: launch") ? SINTER_OK : SINTER_ERR_HIP;
 }
 
@@ -1687,16 +1868,18 @@ int sinter_kv4_read(const sinter_kv4_batch *b, const sinter_heads *k, const sint
     if (!type_ok(type)) return set_error(SINTER_ERR_ARG, "kv4_read: type %d (F32, F16 or BF16)", type);
     if (b->n_seq == 0 || b->n_tok == 0) return SINTER_OK;
     Rows r;
-    r.b = *b; r.type = (uint32_t)type;
+    r.b = *b;
     r.k = k ? *k : sinter_heads{}; r.v = v ? *v : sinter_heads{};
     if (!r.k.p && !r.v.p) return set_error(SINTER_ERR_ARG, "kv4_read: nowhere to write");
     const char *why;
     if ((r.k.p && (why = check_heads(r.k, b->n_tok, b->nkv, b->hd, type))) || (r.v.p && (why = check_heads(r.v, b->n_tok, b->nkv, b->hd, type))))
         return set_error(SINTER_ERR_ARG, "kv4_read: %s", why);
-    r.per = (2 * b->nkv * (b->hd / 16) + 255) / 256;
-    const uint64_t grid = (uint64_t)b->n_tok * r.per;
+    const uint32_t el = type == SINTER_F32 ? 4 : 8, both = r.k.p && r.v.p ? 2 : 1;
+    const uint64_t grid = rows_grid(r, both * b->nkv * (b->hd / el), 256);
     if (grid > (uint64_t)INT32_MAX) return set_error(SINTER_ERR_ARG, "kv4_read: too many tokens");
-    hipLaunchKernelGGL(kv4_read_kernel, dim3((uint32_t)grid), dim3(256), 0, (hipStream_t)stream, r);
+    by_type((uint32_t)type, [&](auto t) {
+        hipLaunchKernelGGL(kv4_read_kernel<decltype(t)::value>, dim3((uint32_t)grid), dim3(256), 0, (hipStream_t)stream, r);
+    });
     return hip_ok(hipGetLastError(), "kv4_read: launch") ? SINTER_OK : SINTER_ERR_HIP;
 }
 
