@@ -401,10 +401,8 @@ void sinter_argmax_ws_destroy(sinter_argmax_ws *dev);
 
 /* ------------------------------------------------------------------ 4-bit paged KV cache */
 /* Operators over a KV cache of 4-bit codes that a batch of sequences shares in
- * pages: the per-token work around SINTER_OP_ATTN_DECODE's (q/k norm and rope,
- * KV append, attention, gate; k0/ops/attn.cuh:119-488) for many sequences and
- * any number of new tokens each.  No counterpart in the reference, whose cache
- * is one sequence's f16 rows.
+ * pages: the steps of SINTER_OP_ATTN_DECODE (q/k norm and rope, KV append,
+ * attention, gate) for many sequences and any number of new tokens each.
  *
  * Cache: K and V are n_pages pages of sinter_kv4_page_bytes each.  In a page,
  * kv head after kv head: page_rows rows of hd / 2 code bytes (byte 16 b + i of
@@ -469,8 +467,8 @@ int sinter_kv4_prep(const sinter_kv4_batch *b, const sinter_kv4_prep_args *a, vo
 
 /* The tokens' k and v rows (nkv heads) quantised into their cache rows: per 32
  * elements m = the first of the largest magnitude, d = m / -8, code = min(15,
- * trunc(x * (1 / d) + 8.5)) in fp32, the scale f16(d) (ggml's
- * quantize_row_q4_0_ref).  Magnitudes saturate at 65504; a NaN makes its
+ * trunc(x * (1 / d) + 8.5)) in fp32, the scale f16(d) (as
+ * Q4_0 rows have them).  Magnitudes saturate at 65504; a NaN makes its
  * block's scale NaN; a scale that rounds to 0 makes the block 0. */
 int sinter_kv4_append(const sinter_kv4_batch *b, const sinter_heads *k, const sinter_heads *v, int type, void *stream);
 
@@ -486,7 +484,8 @@ int sinter_kv4_read(const sinter_kv4_batch *b, const sinter_heads *k, const sint
  * max_q and max_kv bound the new tokens and the rows of every sequence (a
  * sequence over them raises SINTER_E_BAD_SHAPE); ws: sinter_kv4_attn_ws_bytes
  * of device memory, 16-byte aligned (null if 0), used only while the call
- * runs: calls that may overlap need one each. */
+ * runs: calls that may overlap need one each.  out overlaps neither q nor
+ * gate.  Batches whose row counts 31 bits do not hold are refused. */
 typedef struct sinter_kv4_attn_args {
     sinter_heads q, gate, out;   /* nq heads each */
     void *ws;

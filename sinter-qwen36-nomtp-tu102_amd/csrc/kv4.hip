@@ -5,10 +5,10 @@
 //   kv4_prep_kernel    RMSNorm + NEOX RoPE of q and k heads
 //   kv4_append_kernel  k, v rows quantised into the cache's pages
 //   kv4_read_kernel    cache rows back to f32 / f16 / bf16
-//   kv4_split_kernel   attention of 16 (token, head) rows over a chunk of cache rows
-//   kv4_merge_kernel   its chunks' partials of a row joined
-//   kv4_tile_kernel    attention of 128 rows of one sequence over a chunk
-//   kv4_join_kernel    its chunks' partials joined
+//   kv4_split_kernel   attention of 16 (token, head) rows over a part of the cache rows
+//   kv4_merge_kernel   the parts of a row joined
+//   kv4_tile_kernel    attention of 128 or 256 rows of one sequence over a chunk
+//   kv4_join_kernel    its chunks joined
 //
 // A page holds per kv head page_rows rows of codes (hd / 2 bytes; byte 16 b +
 // i of a row holds elements 32 b + i and 32 b + 16 + i in its low and high
@@ -85,10 +85,27 @@ struct Raw4 {
 
 // ------------------------------------------------------------------ the batch
 
+// The first of 64 sequences among which token t's is (wave-uniform), or any if
+// it has none: 64 starts are compared at a time, so that of up to 4096
+// sequences one load finds the 64 (the append of one row of 2048 sequences, 8
+// heads of 128: 18 us, 31 with a look through all of them).
+__device__ __forceinline__ uint32_t seq_base(const sinter_kv4_batch &b, uint32_t t) {
+    const uint32_t lane = threadIdx.x & 63u;
+    uint32_t base = 0, span = b.n_seq;
+    while (span > 64) {
+        const uint32_t stride = (span + 63) / 64, i = base + lane * stride;
+        const bool before = lane * stride < span && b.tok_start[min(i, b.n_seq)] <= (int)t;
+        const uint32_t c = (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(before)), at = c ? (c - 1) * stride : 0u;
+        base += at;
+        span = min(stride, span - at);
+    }
+    return base;
+}
+
 // the sequence that token t belongs to (wave-uniform), or -1
 __device__ __forceinline__ int seq_of(const sinter_kv4_batch &b, uint32_t t) {
     const uint32_t lane = threadIdx.x & 63u;
-    for (uint32_t base = 0; base < b.n_seq; base += 64) {
+    for (uint32_t base = seq_base(b, t); base < b.n_seq; base += 64) {
         const uint32_t i = min(base + lane, b.n_seq - 1u);
         const bool past = base + lane < b.n_seq && b.tok_start[i + 1] > (int)t;
         const uint64_t m = __builtin_amdgcn_ballot_w64(past);
@@ -108,7 +125,7 @@ __device__ __forceinline__ void token_places(const sinter_kv4_batch &b, uint32_t
     const uint32_t lane = threadIdx.x & 63u;
     seq = pos = -1;
     uint32_t k = 0;
-    for (uint32_t base = 0; base < b.n_seq && k < n; base += 64) {
+    for (uint32_t base = seq_base(b, t0); base < b.n_seq && k < n; base += 64) {
         const uint32_t i = min(base + lane, b.n_seq - 1u);
         const int start = b.tok_start[i], stop = b.tok_start[i + 1], len = b.kv_len[i];
         for (; k < n; k++) {
@@ -275,7 +292,7 @@ struct Rows {
 // Four lanes quantise one block of 32, eight elements each: m = the first
 // element of the largest magnitude (saturated at the f16 maximum), d = m / -8,
 // code = min(15, trunc(x / d + 8.5)) by the product with 1 / d, in fp32 with
-// every product and sum rounded (ggml's Q4_0 reference quantiser).  A block
+// every product and sum rounded.  A block
 // whose f16 scale is zero has every code 8; one with a NaN has a NaN scale.
 // A workgroup takes several tokens, whose places are found together, and four
 // blocks' loads at a time.  Bound by instructions (about 200 for a wave's 16
@@ -424,33 +441,41 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Rows a) {
 // ------------------------------------------------------------------ attention
 
 constexpr uint32_t TILE = 32;   // cache rows a tile
-// Tiles a slot of kv4_split_kernel takes at least (two a wave), and the tiles
-// up to which a sequence is not divided (its join would cost more)
-constexpr uint32_t CT_MIN = 8, WHOLE = 16;
+// Of kv4_split_kernel (27B heads, F32): tiles a slot takes at least, one a wave
+// (a reply behind 600 rows: 12.4 us, 8 tiles 14.2, 16 18.6); tiles up to which a
+// segment is not divided (64 replies behind 400 rows: 23 us, up to 8 31; a reply
+// behind 1000: 14, up to 32 24); and the tiles more a slot may get so that it has
+// one segment only (4 to 16 measure alike)
+constexpr uint32_t CT_MIN = 4, WHOLE = 16, OWN_MORE = 8;
 
 struct Attn {
     sinter_kv4_batch b;
     sinter_heads q, gate, out;
-    float *part;     // [slot][2][kv head][row tile][16][hd] unnormalised sums
-    float2 *ml;      // [slot][2][kv head][row tile][16] reference and weight sum
+    float *part;     // [slot][2][kv head][16][hd] unnormalised sums
+    float2 *ml;      // [slot][2][kv head][16] reference and weight sum
     float *tpart;    // kv4_tile_kernel's: [tile][kv head][chunk][tile rows][hd]
     float2 *tml;
-    uint32_t nq, gqa, max_q, max_kv, n_slots, n_mt, type, page_shift;
+    uint32_t nq, gqa, max_q, max_kv, n_slots, type, page_shift;
     uint32_t n_tile, n_split, report;   // kv4_tile_kernel: row tiles and chunks; report the errors of lengths
-    uint32_t split_rows;   // sequences of up to these rows are kv4_split_kernel's (SPLIT_ROWS; 0: it is not launched)
+    uint32_t split_rows;   // sequences of up to these rows are kv4_split_kernel's (0: it is not launched)
     uint32_t gqa_inv;   // ceil(2^32 / gqa), gqa > 1
     float qscale;    // scale * log2(e)
 };
 
 // The sequences of a call go two ways by their rows, (token, q head of a kv
-// head) pairs: up to SPLIT_ROWS of them to kv4_split_kernel, which streams the
-// cache past 16 rows, more to kv4_tile_kernel, whose waves share a tile's codes
-// once unpacked.
-constexpr uint32_t SPLIT_ROWS = 32;
+// head) pairs: few to kv4_split_kernel, which streams the cache past 16 rows,
+// many to kv4_tile_kernel, whose waves share a tile's codes once unpacked.
+// SPLIT_ROWS: up to there the first is the faster one in any batch (8 sequences
+// of 48 rows behind 5000, 27B heads, F32: 52 us, the other 139; 32 of 96 rows
+// behind 2000, bf16: 124 and 143; of 192 rows 207 and 152).  SPLIT_MOST: where
+// all of a batch is little work, which leaves the second's workgroups too few
+// (one sequence of 252 rows behind 1000, F32: 24 us and 41).
+constexpr uint32_t SPLIT_ROWS = 96, SPLIT_MOST = 256;
 
 struct Work {
     int seq, len, tok0, n_new;   // the sequence: rows, first token, tokens (seq < 0: none)
     uint32_t item, first, count; // the item of it, the number of its item 0, its items
+    uint32_t base, before;       // a sequence to look on from, the items before it
 };
 
 // the most rows of a sequence that the launch and the page table have room for
@@ -490,6 +515,8 @@ __device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v) {
     return v;
 }
 
+__device__ __forceinline__ uint32_t wave_sum_u32(uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)wave_scan_u32(v), 63); }
+
 // Of the 64 sequences from `base` on (a lane's: rows, first token, tokens, items
 // c from number lo on), the one that has item `id`, or (by_seq) sequence `id`.
 __device__ __forceinline__ bool pick(Work &w, uint32_t base, uint32_t id, bool by_seq, int len, int t0, int n, uint32_t c,
@@ -509,17 +536,19 @@ __device__ __forceinline__ bool pick(Work &w, uint32_t base, uint32_t id, bool b
 }
 // The sequences' items, count(len, n) each, numbered one sequence after the
 // other: item `id`'s sequence, or (by_seq) sequence `id` with its item 0.
+// from: an earlier result, whose place the search starts at.
 template <class Count>
-__device__ __forceinline__ Work locate(const Attn &a, uint32_t id, bool by_seq, Count count) {
+__device__ __forceinline__ Work locate(const Attn &a, uint32_t id, bool by_seq, Count count, const Work *from = nullptr) {
     Work w;
     w.seq = -1;
-    uint32_t before = 0;
-    for (uint32_t base = 0; base < a.b.n_seq; base += 64) {
+    w.base = from ? from->base : 0u;
+    w.before = from ? from->before : 0u;
+    for (; w.base < a.b.n_seq; w.base += 64) {
         int len, t0, n;
-        load_seq(a, base, false, len, t0, n);
+        load_seq(a, w.base, false, len, t0, n);
         const uint32_t c = n > 0 ? count(len, n) : 0u, sum = wave_scan_u32(c);
-        if (pick(w, base, id, by_seq, len, t0, n, c, before + sum - c)) return w;
-        before += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+        if (pick(w, w.base, id, by_seq, len, t0, n, c, w.before + sum - c)) return w;
+        w.before += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
     }
     return w;
 }
@@ -533,45 +562,78 @@ __device__ __forceinline__ void report_lengths(const Attn &a) {
 
 __device__ __forceinline__ bool is_split(const Attn &a, int n) { return (uint32_t)n * a.gqa <= a.split_rows; }
 
-// kv4_split_kernel's work is the list of its sequences' tiles, one sequence
-// after the other (at least one each), in equal shares: slot i takes tiles [i
-// ct, (i + 1) ct), except that a sequence of up to WHOLE tiles goes undivided
-// to the slot of its first.
-__device__ __forceinline__ uint32_t tiles_of(const Attn &a, int len, int n) {
-    return is_split(a, n) ? max(1u, (min((uint32_t)len, row_cap(a)) + TILE - 1u) / TILE) : 0u;
+// kv4_split_kernel's work is a list of segments, a segment being 16 rows of a
+// sequence and its cache tiles (at least one), those of a sequence one after the
+// other, counted in units of `tiles` tiles; a segment of up to WHOLE tiles is not
+// divided.  Slot i takes units [i share, (i + 1) share), an undivided segment
+// being the slot's that has its first.
+struct Deal { uint32_t total, tiles, share; };
+__device__ __forceinline__ uint32_t row_tiles(const Attn &a, int n) { return n > 0 && is_split(a, n) ? ((uint32_t)n * a.gqa + 15u) / 16u : 0u; }
+__device__ __forceinline__ uint32_t seg_tiles(const Attn &a, int len) { return max(1u, (min((uint32_t)len, row_cap(a)) + TILE - 1u) / TILE); }
+__device__ __forceinline__ uint32_t seg_units(uint32_t tiles, uint32_t per) {
+    return per == 1u ? tiles : tiles <= WHOLE ? 1u : (tiles + per - 1u) / per;
 }
-__device__ __forceinline__ uint32_t all_tiles(const Attn &a) {
-    uint32_t total = 0;
-    for (uint32_t base = 0; base < a.b.n_seq; base += 64) {
-        int len, t0, n;
-        load_seq(a, base, false, len, t0, n);
-        total += (uint32_t)__builtin_amdgcn_readlane((int)wave_scan_u32(n > 0 ? tiles_of(a, len, n) : 0u), 63);
+// x / n rounded up, of uniform values (or a little more where x passes 2^22).
+// Short: a call's first instructions are fetched as they are run, and a
+// microsecond of a reply's 13 was this code's length
+__device__ __forceinline__ uint32_t share_of(uint32_t x, uint32_t n) {
+    uint32_t q = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)((float)x * __builtin_amdgcn_rcpf((float)n)));
+    while (q * n < x) q++;
+    return q;
+}
+// Where it makes the slots little longer a unit is a slot's share: none then has
+// two segments, each with its start and end (8 replies of 4 tokens behind 5000
+// rows, 27B heads, F32: 39.0 us, without 42.4).  Else a unit is a tile, in equal
+// shares; of many segments at least their mean, so that the undivided start
+// where a slot does (64 replies behind 400 rows: 18 us, without 23).
+__device__ __forceinline__ Deal deal_of(const Attn &a, uint32_t total, uint32_t segs) {
+    Deal d = {total, 1, 1};
+    if (segs < a.n_slots) {
+        // (segments' units are at most (total - segs) / tiles + segs)
+        d.tiles = max(CT_MIN, share_of(total - segs, a.n_slots - segs));
+        if (d.tiles <= OWN_MORE || (float)(d.tiles - OWN_MORE) * (float)a.n_slots <= (float)total) return d;
+        d.tiles = 1;
     }
-    return total;
+    d.share = max(1u, share_of(total, a.n_slots));
+    if (segs * a.b.nkv >= 256u) d.share = max(d.share, min(WHOLE, share_of(total, segs)));
+    return d;
 }
-__device__ __forceinline__ uint32_t slot_tiles(const Attn &a, uint32_t total) {
-    return max(CT_MIN, (total + a.n_slots - 1u) / a.n_slots);
+__device__ __forceinline__ Work find_units(const Attn &a, const Deal &d, uint32_t id, bool by_seq, const Work *from = nullptr) {
+    return locate(a, id, by_seq, [&](int len, int n) { return row_tiles(a, n) * seg_units(seg_tiles(a, len), d.tiles); }, from);
 }
-__device__ __forceinline__ Work find_tiles(const Attn &a, uint32_t id, bool by_seq) {
-    return locate(a, id, by_seq, [&](int len, int n) { return tiles_of(a, len, n); });
-}
-// All of it at once, where a lane holds every sequence: the total, the tiles a
-// slot, and the work at slot `id`'s first tile or (by_seq) of sequence `id`
-__device__ __forceinline__ Work first_tiles(const Attn &a, uint32_t id, bool by_seq, uint32_t &total, uint32_t &ct) {
-    if (a.b.n_seq <= 64) {
-        int len, t0, n;
+// The deal, and the work at slot `id`'s first unit or (by_seq) of sequence `id`.
+__device__ __forceinline__ Work deal(const Attn &a, uint32_t id, bool by_seq, Deal &d) {
+    int len, t0, n;
+    if (a.b.n_seq <= 64) {   // (a lane holds every sequence)
         load_seq(a, 0, false, len, t0, n);
-        const uint32_t c = n > 0 ? tiles_of(a, len, n) : 0u, sum = wave_scan_u32(c);
-        total = (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
-        ct = slot_tiles(a, total);
+        const uint32_t mts = row_tiles(a, n), tiles = seg_tiles(a, len);
+        d = deal_of(a, wave_sum_u32(mts * tiles), wave_sum_u32(mts));
+        const uint32_t c = mts * seg_units(tiles, d.tiles), sum = wave_scan_u32(c);
+        d.total = (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
         Work w;
         w.seq = -1;
-        pick(w, 0, by_seq ? id : id * ct, by_seq, len, t0, n, c, sum - c);
+        w.base = w.before = 0;
+        pick(w, 0, by_seq ? id : id * d.share, by_seq, len, t0, n, c, sum - c);
         return w;
     }
-    total = all_tiles(a);
-    ct = slot_tiles(a, total);
-    return find_tiles(a, by_seq ? id : id * ct, by_seq);
+    uint32_t total = 0, segs = 0;
+#pragma unroll 4
+    for (uint32_t base = 0; base < a.b.n_seq; base += 64) {   // (four loads in flight)
+        load_seq(a, base, false, len, t0, n);
+        const uint32_t mts = row_tiles(a, n);
+        total += wave_sum_u32(mts * seg_tiles(a, len));
+        segs += wave_sum_u32(mts);
+    }
+    d = deal_of(a, total, segs);
+    if (d.tiles > 1u) {
+        d.total = 0;
+#pragma unroll 4
+        for (uint32_t base = 0; base < a.b.n_seq; base += 64) {
+            load_seq(a, base, false, len, t0, n);
+            d.total += wave_sum_u32(row_tiles(a, n) * seg_units(seg_tiles(a, len), d.tiles));
+        }
+    }
+    return find_units(a, d, by_seq ? id : id * d.share, by_seq);
 }
 
 // the gated, normalised output of four elements
@@ -638,10 +700,11 @@ __device__ __forceinline__ f16x8 join8(f16x2 a, f16x2 b, f16x2 c, f16x2 d) {
 // largest scale seen, 2^dlog; a new reference leaves the largest at 2^FRESH.
 constexpr float TOP = 15.0f, FRESH = 6.0f;
 
-// Work item: (slot, kv head, tile of 16 rows), a row being a (token, q head of
-// the group) pair, token-major; the slot's sequences one after the other.
-// Each wave streams its own 32-row tiles of a segment (every fourth) through a private double buffer filled by
-// LDS-DMA, so that no barrier stands between the first tile and the last.
+// Work item: (slot, kv head), the slot's segments one after the other: 16 rows,
+// a row being a (token, q head of the group) pair, token-major.  Each wave
+// streams its own 32-row tiles of a segment (every fourth) through a private
+// double buffer filled by LDS-DMA, so that no barrier stands between the first
+// tile and the last.
 //
 // Scores S^T = K Q^T on 16x16x32 f16 MFMA, one per block of 32 dims: the codes
 // are exact in f16, the block's scale multiplies the fp32 sum (one fma), and q
@@ -651,6 +714,11 @@ constexpr float TOP = 15.0f, FRESH = 6.0f;
 // with the keys in that order: P never leaves its lane.  V's operand comes
 // from a transposing LDS read, eight keys' byte of one dim pair per lane; its
 // scales multiply P (per block, in fp32, rounded once to f16, or to two parts).
+//
+// Bound by the cache's bytes and the codes' unpacking about alike: 64 replies
+// with 8600 rows on average (24 heads over 4 of 256, bf16; 635 MB) in 135 us, 4.7
+// TB/s; one behind 131,000 rows (F32; 151 MB) 42 us and 7 to join, where the
+// start and end of the workgroups are a quarter of it.
 template <int HD, int NS>
 __global__ __launch_bounds__(256, 2) void kv4_split_kernel(Attn a) {
     constexpr uint32_t NB = HD / 32, HB = HD / 2, SB = HD / 16, NCH = HB / 16, KC = TILE * HB, SC = TILE * SB;
@@ -660,22 +728,29 @@ __global__ __launch_bounds__(256, 2) void kv4_split_kernel(Attn a) {
     __shared__ float red[2][4][16];
     const uint32_t lane = threadIdx.x & 63u, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t r16 = lane & 15u, g4 = lane >> 4, NKV = a.b.nkv;
-    const uint32_t g = blockIdx.x, slot = blockIdx.y, mt = blockIdx.z;
-    // (a row's token: rows < 32, gqa <= 32, so the product with ceil(2^32 / gqa) has the quotient)
+    const uint32_t g = blockIdx.x, slot = blockIdx.y;
+    uint32_t mt = 0;   // the segment's rows: 16 mt ..
+    // (a row's token: rows <= SPLIT_MOST and gqa <= SPLIT_MOST, so the product with ceil(2^32 / gqa) has the quotient)
     auto tok_of = [&](uint32_t r) { return a.gqa == 1 ? 16 * mt + r : __umulhi(16 * mt + r, a.gqa_inv); };
-    uint32_t total, ct;
-    Work wk = first_tiles(a, slot, false, total, ct);
-    const uint32_t x0 = slot * ct, x1 = min(x0 + ct, total);
+    Deal d;
+    Work wk = deal(a, slot, false, d);
+    const uint32_t x0 = slot * d.share, x1 = min(x0 + d.share, d.total);
     bool again = false;
     for (uint32_t x = x0; x < x1;) {
-    if (x > x0) wk = find_tiles(a, x, false);
+    if (x > x0) {
+        const Work last = wk;
+        wk = find_units(a, d, x, false, &last);
+    }
     if (wk.seq < 0) break;   // (never: x < total)
-    const uint32_t t0 = x - wk.first, t1 = wk.count <= WHOLE ? wk.count : min(x1 - wk.first, wk.count);   // its tiles here
-    const bool ours = t0 == 0 || wk.count > WHOLE, whole = t0 == 0 && t1 == wk.count;
+    const uint32_t tiles = seg_tiles(a, wk.len), units = seg_units(tiles, d.tiles);
+    mt = wk.count == units ? 0u : (x - wk.first) / units;
+    const uint32_t begin = wk.first + mt * units, stop = tiles <= WHOLE ? units : min(x1 - begin, units);
+    const uint32_t t0 = (x - begin) * d.tiles, t1 = tiles <= WHOLE ? tiles : min(stop * d.tiles, tiles);   // the segment's tiles here
+    const bool ours = t0 == 0 || tiles > WHOLE, whole = t0 == 0 && t1 == tiles;
     const uint32_t rec0 = slot * 2 + (x > x0 ? 1u : 0u);
-    x = wk.first + t1;
+    x = begin + stop;
     const uint32_t M = (uint32_t)wk.n_new * a.gqa;
-    if (!ours || 16 * mt >= M) continue;
+    if (!ours) continue;
     if (again) __syncthreads();   // (the last segment's sums have been read)
     again = true;
     const uint32_t rows = min(16u, M - 16 * mt);
@@ -997,33 +1072,55 @@ __global__ __launch_bounds__(256, 2) void kv4_split_kernel(Attn a) {
             const uint32_t tk = tok_of(r);
             store_out(a, wk.tok0 + (int)tk, (g - tk) * a.gqa + 16 * mt + r, e, o, l);
         } else {
-            const size_t rec = (((size_t)rec0 * NKV + g) * a.n_mt + mt) * 16 + r;
+            const size_t rec = ((size_t)rec0 * NKV + g) * 16 + r;
             *reinterpret_cast<f32x4 *>(a.part + rec * HD + e) = o;
             if (e == 0) a.ml[rec] = make_float2(m, l);
         }
     }
     }
-    if ((g | slot | mt) == 0 && w == 0) report_lengths(a);
+    if ((g | slot) == 0 && w == 0) report_lengths(a);
 }
 
-// A sequence divided over slots: out = sum c_i O_i / sum c_i l_i with c_i =
-// exp2(ref_i - max ref) over its segments.  One workgroup per (sequence, kv
-// head, row); wave w takes every NW-th segment, all of its loads in flight for
-// up to 8 NW.
+// A segment divided over slots: out = sum c_i O_i / sum c_i l_i with c_i =
+// exp2(ref_i - max ref) over its parts.  One workgroup per (sequence, kv head,
+// row); wave w takes every NW-th part, all of its loads in flight for up to 8
+// NW.  Latency: 3 us of a few parts, 7 of 128.
 template <int NW>
 __global__ __launch_bounds__(64 * NW) void kv4_merge_kernel(Attn a, uint32_t rows) {
     __shared__ float2 red[NW];   // a wave's reference and weight sum
     __shared__ __attribute__((aligned(16))) float comb[NW][256];
     const uint32_t r = blockIdx.x % rows, sg = blockIdx.x / rows, g = sg % a.b.nkv, lane = threadIdx.x & 63u, HD = a.b.hd;
     const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    uint32_t total, ct;
-    const Work wk = first_tiles(a, sg / a.b.nkv, true, total, ct);
-    if (wk.seq < 0 || wk.count <= WHOLE || r >= (uint32_t)wk.n_new * a.gqa) return;
-    const uint32_t i0 = wk.first / ct, i1 = (wk.first + wk.count - 1u) / ct;
-    if (i0 == i1) return;
-    const uint32_t n = i1 - i0 + 1u, head1 = wk.first > i0 * ct ? 1u : 0u;   // (its first segment: the slot's own first, or its last)
+    // (one wave looks the parts up: sixteen at it would take turns)
+    __shared__ uint32_t place[4];   // parts, the first one's slot, whether that is the slot's second record, first token
+    if (w == 0) {
+        Deal d;
+        const Work wk = deal(a, sg / a.b.nkv, true, d);
+        uint32_t n = 0, i0 = 0, second = 0;
+        if (wk.seq >= 0 && r < (uint32_t)wk.n_new * a.gqa) {
+            const uint32_t tiles = seg_tiles(a, wk.len), units = seg_units(tiles, d.tiles), begin = wk.first + r / 16 * units;
+            i0 = begin;
+            n = begin + units - 1u;
+            if (d.share > 1u) {
+                i0 /= d.share;
+                n /= d.share;
+            }
+            n = tiles > WHOLE ? n - i0 + 1u : 0u;
+            second = begin > i0 * d.share ? 1u : 0u;
+        }
+        if (lane == 0) {
+            place[0] = n;
+            place[1] = i0;
+            place[2] = second;
+            place[3] = (uint32_t)wk.tok0;
+        }
+    }
+    __syncthreads();
+    const uint32_t n = (uint32_t)__builtin_amdgcn_readfirstlane((int)place[0]), i0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)place[1]);
+    const uint32_t head1 = (uint32_t)__builtin_amdgcn_readfirstlane((int)place[2]);
+    if (n < 2) return;
     auto rec = [&](uint32_t c) {
-        return (((size_t)((i0 + c) * 2 + (c == 0 ? head1 : 0u)) * a.b.nkv + g) * a.n_mt + r / 16) * 16 + r % 16;
+        return (((size_t)(i0 + c) * 2 + (c == 0 ? head1 : 0u)) * a.b.nkv + g) * 16 + r % 16;
     };
     float m = REF_NONE, l = 0.0f;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -1069,7 +1166,7 @@ __global__ __launch_bounds__(64 * NW) void kv4_merge_kernel(Attn a, uint32_t row
 #pragma unroll
         for (int j = 0; j < 4; j++) o[j] = fmaf(x[j], c, o[j]);
     }
-    store_out(a, wk.tok0 + (int)(r / a.gqa), g * a.gqa + r % a.gqa, e, o, l);
+    store_out(a, (int64_t)place[3] + r / a.gqa, g * a.gqa + r % a.gqa, e, o, l);
 }
 
 // ------------------------------------------------------------------ many rows
@@ -1082,7 +1179,6 @@ __device__ __forceinline__ Work find_tile(const Attn &a, uint32_t rows, uint32_t
         return is_split(a, n) ? 0u : ((uint32_t)n * a.gqa + rows - 1u) / rows;
     });
 }
-__device__ __forceinline__ uint32_t wave_sum_u32(uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)wave_scan_u32(v), 63); }
 // The id-th tile from the one with the most cache rows down, so that the
 // longest start first (two prompts of 2000 tokens, bf16, 27B heads: sequence
 // after sequence 377 us, so 205).  A sequence with p0 rows before its tokens
@@ -1101,7 +1197,9 @@ __device__ __forceinline__ Work find_ranked_tile(const Attn &a, uint32_t rows, u
     w.seq = -1;
     if (above(0) <= id) return w;
     // above(lo) > id >= above(hi)
-    uint32_t lo = 0, hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)wave_max_f32((float)top) + 1);
+    // (the largest top, exact in fp32 by parts of 24 bits at most)
+    const float m8 = wave_max_f32((float)(top >> 8)), m0 = wave_max_f32((float)(top >> 8) == m8 ? (float)(top & 255u) : 0.0f);
+    uint32_t lo = 0, hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)((((uint32_t)m8 << 8) | (uint32_t)m0) + 1u));
     while (hi - lo > 1) {
         const uint32_t mid = lo + (hi - lo) / 2;
         if (above(mid) > id) lo = mid;
@@ -1123,8 +1221,9 @@ __device__ __forceinline__ Work find_ranked_tile(const Attn &a, uint32_t rows, u
     w.first = wave_sum_u32((threadIdx.x & 63u) < (uint32_t)l ? c : 0u);
     return w;
 }
-// the cache rows a chunk of a tile that sees `seen` rows takes
-constexpr uint32_t CHUNK_MIN = 512;
+// The cache rows a chunk of a tile that sees `seen` rows takes: 128 at least (128
+// rows behind 1000, 27B heads, bf16: 28 us, 512 at least 72, 64 27)
+constexpr uint32_t CHUNK_MIN = 128;
 __device__ __forceinline__ uint32_t chunk_rows(uint32_t seen, uint32_t n_split) {
     return max(CHUNK_MIN, ((seen + n_split - 1u) / n_split + TILE - 1u) / TILE * TILE);
 }
@@ -1151,6 +1250,13 @@ __device__ __forceinline__ uint32_t chunk_rows(uint32_t seen, uint32_t n_split) 
 // A V scale that is not finite would reach rows that do not see its key (0
 // times it): it is 0 in the fragments and named in `odd`, and makes NaN of the
 // block's sums of the rows that do.
+//
+// Bound by the matrix core with the fragment reads and the unpacking beside it,
+// of which the two waves of a SIMD hide little of each other's: 500 tokens of 24
+// heads of 256 over 4 behind 32,000 rows, F32: 1490 us, 266 TF/s and with each
+// product in three parts 800 TF/s of f16 (a large f16 product: 1166); bf16:
+// 630 us, 630 TF/s (without the unpacking 480, without the scores' and sums'
+// products 380).  Two prompts of 2000 tokens, bf16: 168 us, 620 TF/s.
 template <int HD, int T, int NW>
 __global__ __launch_bounds__(64 * NW, T == SINTER_F32 ? 1 : 2) void kv4_tile_kernel(Attn a) {
     constexpr uint32_t NS = T == SINTER_F32 ? 2 : 1, NP = T == SINTER_BF16 ? 1 : 2;   // f16 parts of q (and V), of the weights
@@ -1179,6 +1285,7 @@ __global__ __launch_bounds__(64 * NW, T == SINTER_F32 ? 1 : 2) void kv4_tile_ker
     const Work wk = find_ranked_tile(a, ROWS, id % a.n_tile);
     if (wk.seq < 0) return;
     const uint32_t gt = wk.first + wk.item;
+    if (gt >= a.n_tile) return;   // (sequences that overlap: no room for the chunks' sums)
     const uint32_t M = (uint32_t)wk.n_new * a.gqa, r0 = wk.item * ROWS;
     const int p0 = wk.len - wk.n_new, cap = (int)row_cap(a);
     auto row_pos = [&](uint32_t r) { return p0 + (int)(min(r, M - 1u) / a.gqa); };
@@ -1604,7 +1711,8 @@ __global__ __launch_bounds__(64 * NW, T == SINTER_F32 ? 1 : 2) void kv4_tile_ker
     }
 }
 
-// The chunks of kv4_tile_kernel's rows joined: one wave per (token, q head).
+// The chunks of kv4_tile_kernel's rows joined, one wave per (token, q head):
+// reads each chunk's sums once.
 template <int NW>
 __global__ __launch_bounds__(256) void kv4_join_kernel(Attn a) {
     constexpr uint32_t ROWS = 32 * NW;
@@ -1620,7 +1728,7 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Attn a) {
     const uint32_t g = h / a.gqa, row = i * a.gqa + h % a.gqa, tile = row / ROWS, M = (uint32_t)wk.n_new * a.gqa;
     const int last = wk.len - wk.n_new + (int)(min(tile * ROWS + ROWS - 1u, M - 1u) / a.gqa);
     const uint32_t seen = (uint32_t)max(0, min(last + 1, (int)row_cap(a))), per = chunk_rows(seen, a.n_split);
-    if (seen <= per) return;
+    if (seen <= per || wk.first + tile >= a.n_tile) return;
     const uint32_t n = (seen + per - 1u) / per;
     const size_t rec = (((size_t)(wk.first + tile) * a.b.nkv + g) * a.n_split) * ROWS + row % ROWS;
     float m = REF_NONE, l = 0.0f;
@@ -1642,6 +1750,9 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Attn a) {
 
 bool type_ok(int t) { return t == SINTER_F32 || t == SINTER_F16 || t == SINTER_BF16; }
 int elem_bytes(int t) { return t == SINTER_F32 ? 4 : 2; }
+
+// a launch of `blocks` workgroups has fewer than 2^32 threads
+bool grid_ok(uint64_t blocks, uint32_t threads) { return blocks * threads < ((uint64_t)1 << 32); }
 
 // the rows of a token array: pointer and strides of whole 16-byte units, no two
 // rows overlapping (a stride that is never taken may be anything)
@@ -1689,6 +1800,11 @@ int check_attn(const sinter_kv4_batch *b, const sinter_kv4_attn_args *a) {
         return set_error(SINTER_ERR_ARG, "kv4_attn: scale must be positive and finite");
     if (b->n_seq && b->n_tok && (a->max_q == 0 || a->max_kv == 0 || a->max_kv > (uint32_t)INT32_MAX - 65536u))
         return set_error(SINTER_ERR_ARG, "kv4_attn: max_q %u / max_kv %u", a->max_q, a->max_kv);
+    // (kv4_split_kernel counts its segments' tiles in 32 bits)
+    const uint64_t segs = std::min<uint64_t>((uint64_t)b->n_tok * (a->nq / b->nkv) / 16 + b->n_seq, (uint64_t)b->n_seq * (SPLIT_MOST / 16));
+    if (segs * ((a->max_kv + (uint64_t)TILE - 1) / TILE) > (uint64_t)INT32_MAX || (uint64_t)b->n_tok * a->nq > (uint64_t)INT32_MAX)
+        return set_error(SINTER_ERR_ARG, "kv4_attn: batch too large (%u sequences of up to %u rows, %u tokens of %u heads)", b->n_seq,
+                         a->max_kv, b->n_tok, a->nq);
     return SINTER_OK;
 }
 
@@ -1698,9 +1814,6 @@ int check_attn(const sinter_kv4_batch *b, const sinter_kv4_attn_args *a) {
 // bf16: 684 us against 587)
 constexpr uint32_t tile_waves(bool f32) { return f32 ? 4 : 8; }
 
-// The launches of a batch.  kv4_split_kernel: row tiles a sequence, and slots,
-// as many as run at once.  kv4_tile_kernel: row tiles (at most one
-// partly filled one a sequence) and chunks of the cache rows a tile sees.
 // f(the type as a constant)
 template <class F>
 void by_type(uint32_t type, F f) {
@@ -1720,33 +1833,43 @@ uint64_t rows_grid(Rows &r, uint32_t units, uint32_t wide) {
     return (uint64_t)groups * r.parts;
 }
 
-// (two workgroups a CU by their LDS with heads of 256, by registers three and four with 128 and 64)
+// The launches of a batch.  kv4_split_kernel: row tiles a sequence, and slots,
+// as many as run at once.  kv4_tile_kernel: row tiles (at most one
+// partly filled one a sequence) and chunks of the cache rows a tile sees.
+// Slots: the workgroups that run at once, two a CU by their LDS with heads of
+// 256, three and four by registers with 128 and 64 (a reply behind 130,000 rows,
+// heads of 256, 128: 48 and 42 us; half as many 51 and 52, twice as many 56 and 49)
 uint32_t slots_at_once(uint32_t hd) { return hd == 256 ? 512 : hd == 128 ? 768 : 1024; }
 struct Plan {
-    uint32_t n_mt = 0, n_slots = 0, n_tile = 0, n_split = 1;
+    uint32_t split_rows = 0, merge_rows = 0, n_slots = 0, n_tile = 0, n_split = 1;
     bool split = false, merge = false, join = false;
     uint64_t grid = 0, tile_grid = 0;
     size_t recs = 0, tile_recs = 0;
     size_t bytes(uint32_t hd) const { return (recs + tile_recs) * ((size_t)hd * 4 + 8); }
 };
+// (the work: 16-row segments of all tokens times the cache tiles they may see)
+uint32_t split_rows(const sinter_kv4_batch &b, const sinter_kv4_attn_args &a) {
+    const uint64_t segs = ((uint64_t)b.n_tok * (a.nq / b.nkv) + 15) / 16 * b.nkv;
+    return segs * ((a.max_kv + TILE - 1) / TILE) <= 16384 ? SPLIT_MOST : SPLIT_ROWS;
+}
 Plan make_plan(const sinter_kv4_batch &b, const sinter_kv4_attn_args &a) {
     Plan p;
     const uint32_t gqa = a.nq / b.nkv;
     const uint64_t rows = (uint64_t)std::min(a.max_q, b.n_tok) * gqa;
     // (a sequence that all tokens may belong to, of many rows, is taken whole
     // by kv4_tile_kernel)
-    p.split = gqa <= SPLIT_ROWS && (rows <= SPLIT_ROWS || b.n_seq > 1);
+    p.split_rows = split_rows(b, a);
+    p.split = gqa <= p.split_rows && (rows <= p.split_rows || b.n_seq > 1);
     if (p.split) {
-        p.n_mt = (uint32_t)((std::min<uint64_t>(rows, SPLIT_ROWS) + 15) / 16);
+        p.merge_rows = (uint32_t)std::min<uint64_t>(rows, p.split_rows / gqa * gqa);
         p.merge = a.max_kv > WHOLE * TILE;
-        const uint64_t per = (uint64_t)b.nkv * p.n_mt;
-        const uint64_t most = (uint64_t)b.n_seq * std::max<uint64_t>(1, (a.max_kv + CT_MIN * TILE - 1) / (CT_MIN * TILE));
-        p.n_slots = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(1, slots_at_once(b.hd) / per), most);
-        p.grid = (uint64_t)p.n_slots * b.nkv * p.n_mt;
+        const uint64_t most = (uint64_t)b.n_seq * ((p.merge_rows + 15) / 16) * ((a.max_kv + CT_MIN * TILE - 1) / (CT_MIN * TILE) + 1);
+        p.n_slots = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(1, slots_at_once(b.hd) / b.nkv), most);
+        p.grid = (uint64_t)p.n_slots * b.nkv;
         p.recs = p.merge ? (size_t)p.grid * 32 : 0;
     }
-    if (!p.split || rows > SPLIT_ROWS) {
-        const uint64_t least = p.split ? SPLIT_ROWS / gqa + 1 : 1;   // tokens of a sequence that comes here
+    if (!p.split || rows > p.split_rows) {
+        const uint64_t least = p.split ? p.split_rows / gqa + 1 : 1;   // tokens of a sequence that comes here
         const uint32_t tile_rows = 32 * tile_waves(a.type == SINTER_F32);
         p.n_tile = (uint32_t)((uint64_t)b.n_tok * gqa / tile_rows + std::min<uint64_t>(b.n_seq, b.n_tok / least));
         const uint64_t wgs = (uint64_t)p.n_tile * b.nkv, room = 256;
@@ -1781,7 +1904,7 @@ void launch_attn(const Attn &k, const Plan &p, hipStream_t s) {
         else tile(kv4_tile_kernel<HD, SINTER_BF16, tile_waves(false)>);
     }
     if (p.grid) {
-        const dim3 grid(k.b.nkv, p.n_slots, p.n_mt);
+        const dim3 grid(k.b.nkv, p.n_slots);
         if (f32) hipLaunchKernelGGL((kv4_split_kernel<HD, 2>), grid, dim3(256), 0, s, k);
         else hipLaunchKernelGGL((kv4_split_kernel<HD, 1>), grid, dim3(256), 0, s, k);
     }
@@ -1837,6 +1960,7 @@ int sinter_kv4_prep(const sinter_kv4_batch *b, const sinter_kv4_prep_args *a, vo
     // few tokens: a wave takes one group of heads; many: a workgroup a token
     const uint32_t per = 512 / b->hd, need = ((nq + per - 1) / per + (nk + per - 1) / per + 3) / 4;
     const dim3 grid(b->n_tok, b->n_tok >= 1024 ? 1u : need);
+    if (!grid_ok(b->n_tok, 256)) return set_error(SINTER_ERR_ARG, "kv4_prep: too many tokens");
     by_type(a->type, [&](auto t) {
         hipLaunchKernelGGL(kv4_prep_kernel<decltype(t)::value>, grid, dim3(256), 0, (hipStream_t)stream, p);
     });
@@ -1855,7 +1979,7 @@ int sinter_kv4_append(const sinter_kv4_batch *b, const sinter_heads *k, const si
     Rows r;
     r.b = *b; r.k = *k; r.v = *v;
     const uint64_t grid = rows_grid(r, 2 * b->nkv * (b->hd / 32), 64);
-    if (grid > (uint64_t)INT32_MAX) return set_error(SINTER_ERR_ARG, "kv4_append: too many tokens");
+    if (!grid_ok(grid, 256)) return set_error(SINTER_ERR_ARG, "kv4_append: too many tokens");
     by_type((uint32_t)type, [&](auto t) {
         hipLaunchKernelGGL(kv4_append_kernel<decltype(t)::value>, dim3((uint32_t)grid), dim3(256), 0, (hipStream_t)stream, r);
     });
@@ -1876,7 +2000,7 @@ int sinter_kv4_read(const sinter_kv4_batch *b, const sinter_heads *k, const sint
         return set_error(SINTER_ERR_ARG, "kv4_read: %s", why);
     const uint32_t el = type == SINTER_F32 ? 4 : 8, both = r.k.p && r.v.p ? 2 : 1;
     const uint64_t grid = rows_grid(r, both * b->nkv * (b->hd / el), 256);
-    if (grid > (uint64_t)INT32_MAX) return set_error(SINTER_ERR_ARG, "kv4_read: too many tokens");
+    if (!grid_ok(grid, 256)) return set_error(SINTER_ERR_ARG, "kv4_read: too many tokens");
     by_type((uint32_t)type, [&](auto t) {
         hipLaunchKernelGGL(kv4_read_kernel<decltype(t)::value>, dim3((uint32_t)grid), dim3(256), 0, (hipStream_t)stream, r);
     });
@@ -1900,8 +2024,13 @@ int sinter_kv4_attn(const sinter_kv4_batch *b, const sinter_kv4_attn_args *a, vo
     const size_t need = p.bytes(b->hd);
     if (need && (!a->ws || (uintptr_t)a->ws % 16u || a->ws_bytes < need))
         return set_error(SINTER_ERR_ARG, "kv4_attn: workspace of %zu bytes, 16-byte aligned (sinter_kv4_attn_ws_bytes)", need);
-    if (p.grid > (uint64_t)INT32_MAX || p.tile_grid > (uint64_t)INT32_MAX || (uint64_t)b->n_tok * a->nq > (uint64_t)INT32_MAX ||
-        (p.merge && (uint64_t)b->n_seq * b->nkv * SPLIT_ROWS > (uint64_t)INT32_MAX))
+    const uint32_t out_rows = b->n_tok * a->nq, segs = b->n_seq * ((p.merge_rows + 15) / 16);
+    // Waves of a merging workgroup: sixteen where a row may have many parts (a
+    // reply behind 130,000 rows: 48.5 us, four 54), four where the rows are many
+    // (64 behind 3000: 70 us, sixteen 74)
+    const uint32_t wide = p.n_slots > 32 * segs ? 16 : 4;
+    if (!grid_ok(p.tile_grid, 64 * tile_waves(a->type == SINTER_F32)) || (p.join && !grid_ok((out_rows + 3) / 4, 256)) ||
+        (p.merge && !grid_ok((uint64_t)b->n_seq * b->nkv * p.merge_rows, 64 * wide)))
         return set_error(SINTER_ERR_ARG, "kv4_attn: batch too large");
     Attn k;
     k.b = *b;
@@ -1911,8 +2040,8 @@ int sinter_kv4_attn(const sinter_kv4_batch *b, const sinter_kv4_attn_args *a, vo
     k.ml = reinterpret_cast<float2 *>(k.tpart + p.tile_recs * b->hd);
     k.tml = k.ml + p.recs;
     k.nq = a->nq; k.gqa = a->nq / b->nkv; k.max_q = a->max_q; k.max_kv = a->max_kv;
-    k.n_slots = p.n_slots; k.n_mt = p.n_mt; k.type = a->type;
-    k.n_tile = p.n_tile; k.n_split = p.n_split; k.report = !p.split; k.split_rows = p.split ? SPLIT_ROWS : 0;
+    k.n_slots = p.n_slots; k.type = a->type;
+    k.n_tile = p.n_tile; k.n_split = p.n_split; k.report = !p.split; k.split_rows = p.split ? p.split_rows : 0;
     k.page_shift = (uint32_t)__builtin_ctz(b->page_rows);
     k.qscale = a->scale * 1.44269504088896341f;
     k.gqa_inv = (uint32_t)((((uint64_t)1 << 32) + k.gqa - 1) / k.gqa);
@@ -1921,17 +2050,14 @@ int sinter_kv4_attn(const sinter_kv4_batch *b, const sinter_kv4_attn_args *a, vo
     else if (b->hd == 128) launch_attn<128>(k, p, s);
     else launch_attn<64>(k, p, s);
     if (!hip_ok(hipGetLastError(), "kv4_attn: launch")) return SINTER_ERR_HIP;
-    const uint32_t out_rows = b->n_tok * a->nq;
     if (p.join) {
         if (a->type == SINTER_F32) hipLaunchKernelGGL((kv4_join_kernel<tile_waves(true)>), dim3((out_rows + 3) / 4), dim3(256), 0, s, k);
         else hipLaunchKernelGGL((kv4_join_kernel<tile_waves(false)>), dim3((out_rows + 3) / 4), dim3(256), 0, s, k);
     }
     if (p.merge) {
-        const uint32_t rows = std::min(std::min(a->max_q, b->n_tok) * k.gqa, SPLIT_ROWS / k.gqa * k.gqa);
-        const uint32_t grid = b->n_seq * b->nkv * rows;
-        // (few rows over many slots: a wave a segment or two)
-        if (p.n_slots > 32 * b->n_seq) hipLaunchKernelGGL((kv4_merge_kernel<16>), dim3(grid), dim3(1024), 0, s, k, rows);
-        else hipLaunchKernelGGL((kv4_merge_kernel<4>), dim3(grid), dim3(256), 0, s, k, rows);
+        const dim3 grid(b->n_seq * b->nkv * p.merge_rows);
+        if (wide == 16) hipLaunchKernelGGL((kv4_merge_kernel<16>), grid, dim3(1024), 0, s, k, p.merge_rows);
+        else hipLaunchKernelGGL((kv4_merge_kernel<4>), grid, dim3(256), 0, s, k, p.merge_rows);
     }
     return hip_ok(hipGetLastError(), "kv4_attn: merge launch") ? SINTER_OK : SINTER_ERR_HIP;
 }

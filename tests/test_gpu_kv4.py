@@ -20,8 +20,9 @@ over rows add at most 2^-18 (tiles, waves and chunks of at most 64 each on top
 of the 32 rows of a tile), and a term of a row of n is off by at least f16's
 smallest step, 2^-25 at a largest weight of at least 2^4 / (scale bound): n 2^-26
 of the largest |v|.  All of it in sum w |v|, then the gate's 8 u and the
-type's half step.  Sequences of more than 32 (token, head) rows run on tiles
-unpacked to f16: V's scale * code is rounded (2^-11 of sum w |v|; F32 keeps the
+type's half step.  Sequences of many (token, head) rows (more than 96, or 256
+where the batch is little work) run on tiles unpacked to f16, which the
+tolerance allows from 32 rows on: V's scale * code is rounded (2^-11 of sum w |v|; F32 keeps the
 rest in a second part), and for BF16 K's too, 2^-11 of sum |q k| in a score.
 """
 import ctypes as C
@@ -352,6 +353,65 @@ def test_attention_many_sequences(sn, torch_gpu, n_seq):
     check_attn(b, 2, BF16, q, got, g, 64 ** -0.5)
 
 
+@pytest.mark.parametrize("t", [F32, BF16])
+def test_attention_many_sequences_of_many_rows(sn, torch_gpu, t):
+    """More than 64 sequences, prompts among them, empty ones between."""
+    rng = np.random.default_rng(8)
+    new = rng.integers(0, 3, 90)
+    new[[2, 40, 41, 70, 89]] = [50, 20, 33, 140, 17]
+    kv = new + rng.integers(0, 60, 90)
+    kv[[5, 41, 70]] = [300, 700, 140]
+    b, q, g, got = run_attn(sn, torch_gpu, t, 2, 1, 64, 16, list(new), list(kv), True, 18)
+    check_attn(b, 2, t, q, got, g, 64 ** -0.5)
+
+
+@pytest.mark.parametrize("t,nq,new,kv", [(BF16, 40, [1, 0, 3, 1], [70, 9, 900, 1]), (F32, 33, [1, 1], [600, 31]), (F16, 256, [1, 2], [33, 2])])
+def test_attention_large_groups(sn, torch_gpu, t, nq, new, kv):
+    """More q heads to a kv head than the split kernel's rows."""
+    b, q, g, got = run_attn(sn, torch_gpu, t, nq, 1, 64, 32, new, kv, False, 19)
+    check_attn(b, nq, t, q, got, g, 64 ** -0.5)
+
+
+@pytest.mark.parametrize("n_seq", [300, 4500])
+def test_batches_of_many_sequences(sn, torch_gpu, n_seq):
+    """Replies of thousands of sequences, some without a token, and prompts of
+    hundreds (several tokens a workgroup, across sequences): stored, read back
+    and attended to."""
+    torch = torch_gpu
+    rng = np.random.default_rng(n_seq)
+    new = rng.integers(0, 60, n_seq) if n_seq < 1000 else rng.integers(0, 3, n_seq)
+    kv = np.maximum(new + rng.integers(-1, 5, n_seq), 0)
+    b = Batch(sn, torch, list(new), list(kv), 16, 1, 64, pad=5, seed=n_seq)
+    x = [rng.standard_normal((b.n_tok, 1, 64)).astype(np.float32) for _ in range(2)]
+    dev = [torch.from_numpy(a).to("cuda") for a in x]
+    print(f"{n_seq} sequences, {b.n_tok} tokens", flush=True)
+    L, r, st = sn.lib(), b.rec(), stream(torch)
+    ok(sn, L.sinter_kv4_append(C.byref(r), C.byref(heads(sn, dev[0])), C.byref(heads(sn, dev[1])), F32, st), torch)
+    pos = ref.positions(b.tok_start, b.kv_len, b.n_tok)
+    want = [b.kc.copy(), b.vc.copy()]
+    back = [np.full((b.n_tok, 1, 64), 3.0, np.float32) for _ in range(2)]
+    for i in range(2):
+        code, d16 = ref.quantise(x[i])
+        for j, (s, p) in enumerate(pos):
+            if s >= 0 and p >= 0:
+                ref.put(want[i], b.pages[s, p // 16], p % 16, 0, 16, 1, 64, code[j, 0], d16[j, 0])
+                back[i][j, 0] = ref.values(code[j, 0], d16[j, 0])
+        assert np.array_equal(b.d["kc" if i == 0 else "vc"].cpu().numpy(), want[i])
+    out = [torch.full((b.n_tok, 1, 64), 3.0, device="cuda") for _ in range(2)]
+    ok(sn, L.sinter_kv4_read(C.byref(r), C.byref(heads(sn, out[0])), C.byref(heads(sn, out[1])), F32, st), torch)
+    for i in range(2):
+        assert np.array_equal(out[i].cpu().numpy(), back[i])
+    # attention to the rows of this call (the rows before them: as they are)
+    b.kc, b.vc = want
+    b.fill_rows(n_seq)
+    q = rng.standard_normal((b.n_tok, 2, 64)).astype(np.float32)
+    (_, qv), (_, ov) = strided(torch, q, BF16), strided(torch, np.full(q.shape, 3.0, np.float32), BF16)
+    a, ws = attn_args(sn, torch, b, 2, BF16, qv, ov)
+    ok(sn, L.sinter_kv4_attn(C.byref(b.rec()), C.byref(a), st), torch)
+    check_attn(b, 2, BF16, qv.double().cpu().numpy(), ov.float().cpu().numpy(), None, 64 ** -0.5,
+               only=set(range(0, b.n_tok, 7)))
+
+
 @pytest.mark.parametrize("t", [F32, F16, BF16])
 @pytest.mark.parametrize("toks", [2, 30])
 def test_attention_magnitudes(sn, torch_gpu, t, toks):
@@ -420,6 +480,94 @@ def test_attention_nonfinite_query_stays_alone(sn, torch_gpu, n):
     fine = np.ones((n, 2), bool)
     fine[1, 0] = fine[2, 1] = False
     assert np.isfinite(got[fine]).all()
+
+
+# More than 256 rows a sequence, beside shorter ones: the kernel for many rows
+MANY = [
+    (F32, 16, 1, 256, 16, [20, 1, 40], [100, 30, 41], True), (BF16, 32, 2, 128, 64, [33, 2], [600, 2], False),
+    (F16, 16, 1, 64, 16, [18, 70], [18, 400], True), (F16, 64, 2, 256, 32, [9], [40], False),
+    (BF16, 18, 1, 256, 16, [40], [33], True), (F32, 256, 1, 128, 16, [2, 1], [130, 1], False),
+    (F32, 40, 2, 64, 128, [17, 0, 14], [1500, 3, 14], False), (BF16, 6, 1, 64, 16, [50, 3], [1400, 700], True),
+    (F16, 3, 1, 128, 32, [100, 1], [100, 900], False), (BF16, 2, 2, 256, 16, [300], [301], False),
+]
+
+
+@pytest.mark.parametrize("t,nq,nkv,hd,page,new,kv,gated", MANY)
+def test_attention_of_many_rows(sn, torch_gpu, t, nq, nkv, hd, page, new, kv, gated):
+    b, q, g, got = run_attn(sn, torch_gpu, t, nq, nkv, hd, page, new, kv, gated, 60 + hd + nq)
+    check_attn(b, nq, t, q, got, g, hd ** -0.5)
+
+
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+def test_many_rows_magnitudes(sn, torch_gpu, t):
+    test_attention_magnitudes(sn, torch_gpu, t, 80)
+
+
+@pytest.mark.parametrize("nan", [0x7e00, 0x7c00])
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+def test_many_rows_not_seen_stay_out(sn, torch_gpu, nan, t):
+    test_attention_rows_not_seen_stay_out(sn, torch_gpu, nan, t, 70)
+
+
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+def test_many_rows_nonfinite_query_stays_alone(sn, torch_gpu, t):
+    torch = torch_gpu
+    b = Batch(sn, torch, [20], [70], 16, 1, 64, seed=3)
+    b.fill_rows(5)
+    q = np.random.default_rng(1).standard_normal((20, 20, 64)).astype(np.float32)
+    q[1, 0, 7] = np.nan
+    q[2, 1, 9] = np.inf
+    (_, qv), (_, ov) = strided(torch, q, t), strided(torch, np.zeros_like(q), t)
+    a, ws = attn_args(sn, torch, b, 20, t, qv, ov)
+    ok(sn, sn.lib().sinter_kv4_attn(C.byref(b.rec()), C.byref(a), stream(torch)), torch)
+    got = ov.float().cpu().numpy()
+    assert np.isnan(got[1, 0]).all()
+    fine = np.ones((20, 20), bool)
+    fine[1, 0] = fine[2, 1] = False
+    assert np.isfinite(got[fine]).all()
+
+
+@pytest.mark.parametrize("page", [16, 64])
+def test_many_rows_missing_pages(sn, torch_gpu, page):
+    torch = torch_gpu
+    b = Batch(sn, torch, [2, 20], [60, 90], page, 1, 64, seed=3)
+    b.fill_rows(5)
+    q = np.random.default_rng(1).standard_normal((22, 20, 64)).astype(np.float32)
+    (_, qv), (_, ov) = strided(torch, q, F32), strided(torch, np.zeros_like(q), F32)
+    b.pages[1, 0] = b.n_pages
+    b.up()
+    a, ws = attn_args(sn, torch, b, 20, F32, qv, ov)
+    sn.check(sn.lib().sinter_kv4_attn(C.byref(b.rec()), C.byref(a), stream(torch)), "attn")
+    torch.cuda.synchronize()
+    assert sn.op_error() == (sn.E_BAD_SHAPE, 1)
+    got = ov.cpu().numpy()
+    check_attn(b, 20, F32, q.astype(np.float64), got, None, 0.125, only=(0, 1))
+    for j in (2, 21):
+        rows = range(page, 90 - 20 + (j - 2) + 1)   # (without the first page's)
+        k, v = (np.array([ref.get(c, b.pages[1, r // page], r % page, 0, page, 1, 64) for r in rows]).reshape(-1, 64) for c in (b.kc, b.vc))
+        want, mag, _ = ref.attention(q[j, 7].astype(np.float64), k, v, 0.125)
+        assert np.abs(got[j, 7] - want).max() <= 2.0 ** -15 * mag.max()
+
+
+@pytest.mark.parametrize("what", ["max_q", "max_kv", "tokens"])
+def test_many_rows_over_the_bounds(sn, torch_gpu, what):
+    torch = torch_gpu
+    b = Batch(sn, torch, [1, 30], [30, 600], 16, 1, 64, seed=3)
+    b.fill_rows(5)
+    q = np.random.default_rng(1).standard_normal((31, 16, 64)).astype(np.float32)
+    kw = dict(max_q=30, max_kv=700)
+    if what == "tokens":
+        b.tok_start[2] = 90
+        b.up()
+    else:
+        kw[what] -= 150 if what == "max_kv" else 4
+    (_, qv), (_, ov) = strided(torch, q, BF16), strided(torch, np.zeros_like(q), BF16)
+    a, ws = attn_args(sn, torch, b, 16, BF16, qv, ov, **kw)
+    sn.check(sn.lib().sinter_kv4_attn(C.byref(b.rec()), C.byref(a), stream(torch)), "attn")
+    torch.cuda.synchronize()
+    assert sn.op_error() == (sn.E_BAD_SHAPE, 1)
+    b.tok_start[2] = 31
+    check_attn(b, 16, BF16, qv.double().cpu().numpy(), ov.float().cpu().numpy(), None, 0.125, only=(0,))
 
 
 # ---------------------------------------------------------------- errors seen on the device
@@ -594,12 +742,19 @@ def test_prompts_then_replies(sn, torch_gpu, t, nq, nkv, hd, page):
 def test_graph_replays_follow_the_lengths(sn, torch_gpu):
     """One captured step replayed as the sequences grow, the program's own
     eager work in between; every replay equal to the eager step, bit for bit."""
-    torch = torch_gpu
-    r = Replies(sn, torch, F32, 6, 2, 64, 16, [20, 500], 40, seed=5)
-    r.buffers([20, 500])
+    replay_steps(sn, torch_gpu, 6, 2, [20, 500], [1, 1])
+
+
+def test_graph_replays_of_many_rows(sn, torch_gpu):
+    replay_steps(sn, torch_gpu, 16, 1, [20, 300], [1, 20])
+
+
+def replay_steps(sn, torch, nq, nkv, first, step):
+    r = Replies(sn, torch, F32, nq, nkv, 64, 16, first, 40, seed=5)
+    r.buffers(first)
     r.launch()
     r.check()
-    r.buffers([1, 1])
+    r.buffers(step)
     r.launch()
     torch.cuda.synchronize()
     g = torch.cuda.CUDAGraph()
@@ -653,6 +808,20 @@ def test_same_bits_every_time(sn, torch_gpu):
     for _ in range(5):
         out = torch.zeros_like(q)
         a, ws = attn_args(sn, torch, b, 8, F32, q, out)
+        ok(sn, sn.lib().sinter_kv4_attn(C.byref(b.rec()), C.byref(a), stream(torch)), torch)
+        first = out if first is None else first
+        assert torch.equal(first, out)
+
+
+def test_same_bits_every_time_of_many_rows(sn, torch_gpu):
+    torch = torch_gpu
+    b = Batch(sn, torch, [2, 70, 90], [1800, 900, 700], 64, 2, 64, seed=2)
+    b.fill_rows(3)
+    q = torch.randn(162, 8, 64, device="cuda", dtype=torch.bfloat16)
+    first = None
+    for _ in range(5):
+        out = torch.zeros_like(q)
+        a, ws = attn_args(sn, torch, b, 8, BF16, q, out)
         ok(sn, sn.lib().sinter_kv4_attn(C.byref(b.rec()), C.byref(a), stream(torch)), torch)
         first = out if first is None else first
         assert torch.equal(first, out)

@@ -115,6 +115,20 @@ def test_bad_attention(sn, kw):
     assert L.sinter_kv4_attn_ws_bytes(C.byref(b), C.byref(attn(sn, **kw))) == 0
 
 
+@pytest.mark.parametrize("bk,ak", [(dict(n_seq=65536), dict(max_kv=1 << 22)), (dict(n_tok=1 << 30), dict()),
+                                   (dict(n_seq=65536, n_tok=1 << 20, nkv=256), dict(nq=1024, max_kv=4096))])
+def test_attention_too_large(sn, bk, ak):
+    """Counts that 32 bits, or a launch, do not hold."""
+    L, b = sn.lib(), batch(sn, **bk)
+    q = rows(sn, ld=1 << 20)
+    refused(sn, L.sinter_kv4_attn(C.byref(b), C.byref(attn(sn, q=q, out=q, **ak)), None), "too large")
+
+
+def test_too_many_tokens(sn):
+    L, b = sn.lib(), batch(sn, n_tok=1 << 25)
+    refused(sn, L.sinter_kv4_prep(C.byref(b), C.byref(prep(sn)), None), "too many")
+
+
 def test_workspace(sn):
     L, b = sn.lib(), batch(sn)
     a = attn(sn, max_kv=5000)
