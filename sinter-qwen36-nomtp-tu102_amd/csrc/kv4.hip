@@ -1251,12 +1251,11 @@ __device__ __forceinline__ uint32_t chunk_rows(uint32_t seen, uint32_t n_split) 
 // times it): it is 0 in the fragments and named in `odd`, and makes NaN of the
 // block's sums of the rows that do.
 //
-// Bound by the matrix core with the fragment reads and the unpacking beside it,
-// of which the two waves of a SIMD hide little of each other's: 500 tokens of 24
-// heads of 256 over 4 behind 32,000 rows, F32: 1490 us, 266 TF/s and with each
-// product in three parts 800 TF/s of f16 (a large f16 product: 1166); bf16:
-// 630 us, 630 TF/s (without the unpacking 480, without the scores' and sums'
-// products 380).  Two prompts of 2000 tokens, bf16: 168 us, 620 TF/s.
+// Bound by a wave's instructions and waits beside the matrix core, which is busy
+// a third of the time: 500 tokens of 24 heads of 256 over 4 behind 32,000 rows,
+// F32: 1344 us, 295 TF/s and with each product in three parts 885 TF/s of f16 (a
+// large f16 product: 1166); bf16: 530 us, 750 TF/s.  Two prompts of 2000 tokens,
+// bf16: 163 us, 640 TF/s.
 template <int HD, int T, int NW>
 __global__ __launch_bounds__(64 * NW, T == SINTER_F32 ? 1 : 2) void kv4_tile_kernel(Attn a) {
     constexpr uint32_t NS = T == SINTER_F32 ? 2 : 1, NP = T == SINTER_BF16 ? 1 : 2;   // f16 parts of q (and V), of the weights
@@ -1427,85 +1426,71 @@ __global__ __launch_bounds__(64 * NW, T == SINTER_F32 ? 1 : 2) void kv4_tile_ker
                  });
         }
     };
-    auto unpack = [&](int j, const In &in) {
+    // Tile j's unpacking by the wave, in PIECES pieces.  MIX: F32's one wave a
+    // SIMD puts them between the matrix instructions of the tile before (500
+    // tokens behind 32,000 rows, heads of 256 and 128: 1344 and 1031 us, before
+    // them 1390 and 1163).  The two waves a SIMD of 16-bit types take turns
+    // instead, one unpacking before, one behind its tile's work (two prompts of
+    // 2000 tokens, bf16: 163 us, MIX 171).
+    constexpr uint32_t PIECES = 6 * BPW;
+    constexpr bool MIX = NS == 2;
+    constexpr uint32_t PD = NS == 2 && HD < 256 ? 3 : 2;   // slices read ahead of the matrix core (F32, heads of 128: 2 % faster with 3, of 256 no more)
+    struct Half { i32x2 x; u32x4 d; } half;   // (V's codes and scales, from piece to piece)
+    auto unpack = [&](int j, In &in, uint32_t piece, uint32_t ln) {
         if (ACT < NW && w >= ACT) return;
-        uint32_t ln = lane;
-        asm volatile("" : "+v"(ln));   // (opaque, as in issue)
-        const uint32_t l32 = ln & 31u, hf = ln >> 5;
+        const uint32_t l32 = ln & 31u, hf = ln >> 5, r16 = ln & 15u, g4 = ln >> 4, i = piece / 6, b = BPW * w + i;
+        // (V's read on its way while K is taken apart)
+        const uint32_t part = piece % 6 == 1 ? 3 : piece % 6 == 2 ? 1 : piece % 6 == 3 ? 2 : piece % 6;
         LDS unsigned char *B = F + (j & 1) * BUF;
         const LDS unsigned char *V = R + (j & 1) * KC;
-        const bool real = c0 + j * (int)TILE + (int)l32 < end && !(in.holes >> (l32 >> 4) & 1u);
-        const uint32_t r16 = ln & 15u, g4 = ln >> 4;
+        auto codes = [&](uint32_t x0, uint32_t x1, bool hi, f16x2(&o)[4]) {
+            o[0] = hi ? code_pair_hi(x0) : code_pair_lo(x0);
+            o[1] = hi ? code_pair_hi(x0 >> 8) : code_pair_lo(x0 >> 8);
+            o[2] = hi ? code_pair_hi(x1) : code_pair_lo(x1);
+            o[3] = hi ? code_pair_hi(x1 >> 8) : code_pair_lo(x1 >> 8);
+        };
+        // codes times scales to `to` and, for F32, what the rounding leaves to `rest`
+        auto put = [&](const f16x2(&c)[4], const f16x2(&d)[4], LDS unsigned char *to, LDS unsigned char *rest) {
+            f16x2 p[4], r[4];
 #pragma unroll
-        for (uint32_t i = 0; i < BPW; i++) {
-            const uint32_t b = BPW * w + i;
+            for (int k = 0; k < 4; k++) {
+                p[k] = c[k] * d[k];
+                if constexpr (NS == 2) r[k] = __builtin_elementwise_fma(c[k], d[k], -p[k]);
+            }
+            *reinterpret_cast<LDS f16x8 *>(to) = join8(p[0], p[1], p[2], p[3]);
+            if constexpr (NS == 2) *reinterpret_cast<LDS f16x8 *>(rest) = join8(r[0], r[1], r[2], r[3]);
+        };
+        f16x2 c[4];
+        if (part == 0) {
             // V scales in the operand's key order (read back below by this wave alone): key 16 s + 4 h + x (x < 4), 8 + x (x >= 4) of group 2 s + h
-            const uint32_t vb = real ? in.sc[i] >> 16 : 0u;
+            if (c0 + j * (int)TILE + (int)l32 >= end || (in.holes >> (l32 >> 4) & 1u)) in.sc[i] = 0;   // (no such row)
+            const uint32_t vb = in.sc[i] >> 16;
             const bool fin = (vb & 0x7c00u) != 0x7c00u;
             const uint64_t bad = __builtin_amdgcn_ballot_w64(!fin);
             if (ln == 0) odd[j & 1][b] = (uint32_t)bad;
-            {
-                const uint32_t grp = 2 * (l32 >> 4) + ((l32 >> 2) & 1u), x = (l32 & 3u) + ((l32 >> 1) & 4u);
-                const uint32_t at = (x & 4) | ((x & 1) << 1) | ((x >> 1) & 1);   // 0 2 1 3 4 6 5 7
-                ((LDS u16a *)vsc)[b * 32 + grp * 8 + at] = (uint16_t)(fin ? vb : 0u);
+            const uint32_t grp = 2 * (l32 >> 4) + ((l32 >> 2) & 1u), x = (l32 & 3u) + ((l32 >> 1) & 4u);
+            const uint32_t at = (x & 4) | ((x & 1) << 1) | ((x >> 1) & 1);   // 0 2 1 3 4 6 5 7
+            ((LDS u16a *)vsc)[b * 32 + grp * 8 + at] = (uint16_t)(fin ? vb : 0u);
+            if (KX && hf == 0) ((LDS u16a *)(B + KF + NS * VF))[b * 32 + l32] = (uint16_t)in.sc[i];
+        } else if (part < 3) {   // K's elements 0..15 of the block, 16..31
+            LDS unsigned char *to = B + (2 * b + part - 1) * 1024 + 16 * ln;
+            codes(in.k[i].x, in.k[i].y, part == 2, c);
+            if constexpr (KX) {
+                *reinterpret_cast<LDS f16x8 *>(to) = join8(c[0], c[1], c[2], c[3]);
+            } else {
+                const _Float16 d = __builtin_bit_cast(_Float16, (uint16_t)in.sc[i]);
+                const f16x2 dd[4] = {{d, d}, {d, d}, {d, d}, {d, d}};
+                put(c, dd, to, to + KF / 2);
             }
-        }
-#pragma unroll
-        for (uint32_t i = 0; i < BPW; i++) {
-            const uint32_t b = BPW * w + i;
-            f16x2 kl[4] = {code_pair_lo(in.k[i].x), code_pair_lo(in.k[i].x >> 8), code_pair_lo(in.k[i].y), code_pair_lo(in.k[i].y >> 8)};
-            f16x2 kh[4] = {code_pair_hi(in.k[i].x), code_pair_hi(in.k[i].x >> 8), code_pair_hi(in.k[i].y), code_pair_hi(in.k[i].y >> 8)};
-            if constexpr (!KX) {
-                const _Float16 d = __builtin_bit_cast(_Float16, (uint16_t)(real ? in.sc[i] : 0u));
-                const f16x2 dd = {d, d};
-                f16x2 rl[4], rh[4];   // (F32: what the rounded products leave)
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    const f16x2 l = kl[c] * dd, h = kh[c] * dd;
-                    if constexpr (NS == 2) {
-                        rl[c] = __builtin_elementwise_fma(kl[c], dd, -l);
-                        rh[c] = __builtin_elementwise_fma(kh[c], dd, -h);
-                    }
-                    kl[c] = l;
-                    kh[c] = h;
-                }
-                if constexpr (NS == 2) {
-                    *reinterpret_cast<LDS f16x8 *>(B + KF / 2 + (2 * b) * 1024 + 16 * ln) = join8(rl[0], rl[1], rl[2], rl[3]);
-                    *reinterpret_cast<LDS f16x8 *>(B + KF / 2 + (2 * b + 1) * 1024 + 16 * ln) = join8(rh[0], rh[1], rh[2], rh[3]);
-                }
-            } else if (hf == 0) {
-                ((LDS u16a *)(B + KF + NS * VF))[b * 32 + l32] = (uint16_t)(real ? in.sc[i] : 0u);
-            }
-            *reinterpret_cast<LDS f16x8 *>(B + (2 * b) * 1024 + 16 * ln) = join8(kl[0], kl[1], kl[2], kl[3]);
-            *reinterpret_cast<LDS f16x8 *>(B + (2 * b + 1) * 1024 + 16 * ln) = join8(kh[0], kh[1], kh[2], kh[3]);
-            // V: lane r16 of group g4 gets byte r16 of the group's eight keys
+        } else if (part == 3) {   // V: lane r16 of group g4 gets byte r16 of the group's eight keys
             const uint32_t kr = r16 >> 1, vr = 16 * (g4 >> 1) + 4 * (g4 & 1u) + (kr & 3u) + 8 * (kr >> 2);
-            const i32x2 x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((LDS i32x2 *)(V + vr * HB + 16 * (b ^ swz(vr)) + 8 * (r16 & 1u)));
-            const u32x4 dp = *reinterpret_cast<const LDS u32x4 *>((const LDS uint16_t *)vsc + b * 32 + g4 * 8);
-            const uint32_t x0 = (uint32_t)x.x, x1 = (uint32_t)x.y;
-            const f16x2 vl[4] = {code_pair_lo(x0), code_pair_lo(x0 >> 8), code_pair_lo(x1), code_pair_lo(x1 >> 8)};
-            const f16x2 vh[4] = {code_pair_hi(x0), code_pair_hi(x0 >> 8), code_pair_hi(x1), code_pair_hi(x1 >> 8)};
-            f16x2 hl[4], hh[4];
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                const f16x2 d = pair_of(dp[c]);
-                hl[c] = vl[c] * d;
-                hh[c] = vh[c] * d;
-            }
-            LDS unsigned char *vo = B + KF + b * 2048 + g4 * 512 + 16 * r16;
-            *reinterpret_cast<LDS f16x8 *>(vo) = join8(hl[0], hl[1], hl[2], hl[3]);
-            *reinterpret_cast<LDS f16x8 *>(vo + 256) = join8(hh[0], hh[1], hh[2], hh[3]);
-            if constexpr (NS == 2) {
-                f16x2 ll[4], lh[4];
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    const f16x2 d = pair_of(dp[c]);
-                    ll[c] = __builtin_elementwise_fma(vl[c], d, -hl[c]);
-                    lh[c] = __builtin_elementwise_fma(vh[c], d, -hh[c]);
-                }
-                *reinterpret_cast<LDS f16x8 *>(vo + VF) = join8(ll[0], ll[1], ll[2], ll[3]);
-                *reinterpret_cast<LDS f16x8 *>(vo + VF + 256) = join8(lh[0], lh[1], lh[2], lh[3]);
-            }
+            half.x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((LDS i32x2 *)(V + vr * HB + 16 * (b ^ swz(vr)) + 8 * (r16 & 1u)));
+            half.d = *reinterpret_cast<const LDS u32x4 *>((const LDS uint16_t *)vsc + b * 32 + g4 * 8);
+        } else {   // its elements 0..15 of the block, 16..31
+            LDS unsigned char *to = B + KF + b * 2048 + g4 * 512 + 16 * r16 + (part == 5 ? 256 : 0);
+            const f16x2 d[4] = {pair_of(half.d[0]), pair_of(half.d[1]), pair_of(half.d[2]), pair_of(half.d[3])};
+            codes((uint32_t)half.x.x, (uint32_t)half.x.y, part == 5, c);
+            put(c, d, to, to + VF);
         }
     };
 
@@ -1522,9 +1507,19 @@ __global__ __launch_bounds__(64 * NW, T == SINTER_F32 ? 1 : 2) void kv4_tile_ker
         }
     };
     pin();
-    auto compute = [&](int j, uint32_t holes) {
+    auto fetch = [&](int j, In &in) {
+        uint32_t ln = lane;
+        asm volatile("" : "+v"(ln));   // (opaque, as in issue)
+#pragma unroll
+        for (uint32_t p = 0; p < PIECES; p++) unpack(j + 1, in, p, ln);
+        if (j + 2 < n_tile) issue(j + 2, in);
+    };
+    auto compute = [&](int j, uint32_t holes, In &in) {
         const int row0 = c0 + j * (int)TILE;
-        if (row0 >= wmax) return;   // (uniform) no row of the wave sees the tile
+        if (row0 >= wmax) {   // (uniform) no row of the wave sees the tile
+            if constexpr (MIX) fetch(j, in);
+            return;
+        }
         uint32_t ln = lane;
         asm volatile("" : "+v"(ln));   // (opaque, as in issue)
         const uint32_t hf = ln >> 5;
@@ -1533,23 +1528,27 @@ __global__ __launch_bounds__(64 * NW, T == SINTER_F32 ? 1 : 2) void kv4_tile_ker
         auto q_at = [&](uint32_t m) { return m < QR ? Q[0][m] : ((const LDS f16x8 *)qx)[(w * QL + m - QR) * 64 + ln]; };
         f32x16 S = {0.0f};
         if constexpr (!KX) {
-            f16x8 kf[3], kr[3];
+            f16x8 kf[PD + 1], kr[PD + 1];
 #pragma unroll
-            for (uint32_t m = 0; m < 2; m++) {
+            for (uint32_t m = 0; m < PD; m++) {
                 kf[m] = fr(m * 1024);
                 if constexpr (NS == 2) kr[m] = fr(KF / 2 + m * 1024);
             }
 #pragma unroll
             for (uint32_t m = 0; m < 2 * NB; m++) {
-                const f16x8 k = kf[m % 3], r = kr[m % 3];
-                if (m + 2 < 2 * NB) {   // (two slices ahead of the matrix core)
-                    kf[(m + 2) % 3] = fr((m + 2) * 1024);
-                    if constexpr (NS == 2) kr[(m + 2) % 3] = fr(KF / 2 + (m + 2) * 1024);
+                const f16x8 k = kf[m % (PD + 1)], r = kr[m % (PD + 1)];
+                if (m + PD < 2 * NB) {
+                    kf[(m + PD) % (PD + 1)] = fr((m + PD) * 1024);
+                    if constexpr (NS == 2) kr[(m + PD) % (PD + 1)] = fr(KF / 2 + (m + PD) * 1024);
                 }
                 S = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q_at(m), S, 0, 0, 0);
                 if constexpr (NS == 2) {
                     S = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, Q[NS - 1][m], S, 0, 0, 0);
                     S = __builtin_amdgcn_mfma_f32_32x32x16_f16(r, Q[0][m], S, 0, 0, 0);
+                }
+                if constexpr (MIX) {
+#pragma unroll
+                    for (uint32_t p = m * PIECES / (2 * NB); p < (m + 1) * PIECES / (2 * NB); p++) unpack(j + 1, in, p, ln);
                 }
                 sched_fence();
             }
@@ -1570,8 +1569,13 @@ __global__ __launch_bounds__(64 * NW, T == SINTER_F32 ? 1 : 2) void kv4_tile_ker
                     S[4 * i + 2] = fmaf(t[4 * i + 2], (float)d1.x, S[4 * i + 2]);
                     S[4 * i + 3] = fmaf(t[4 * i + 3], (float)d1.y, S[4 * i + 3]);
                 }
+                if constexpr (MIX) {
+#pragma unroll
+                    for (uint32_t p = b * PIECES / NB; p < (b + 1) * PIECES / NB; p++) unpack(j + 1, in, p, ln);
+                }
             }
         }
+        if (MIX && j + 2 < n_tile) issue(j + 2, in);
         const bool masked = __builtin_amdgcn_readfirstlane(row0 + (int)TILE > wmin || holes != 0 ? 1 : 0) != 0;
         auto sees = [&](uint32_t v) {
             return row0 + (int)(8 * (v >> 2) + 4 * hf + (v & 3u)) < my_vis && !(holes >> (v >> 3) & 1u);
@@ -1622,19 +1626,19 @@ __global__ __launch_bounds__(64 * NW, T == SINTER_F32 ? 1 : 2) void kv4_tile_ker
                     P[0][s][k + 1] = (_Float16)p1;
                 }
             }
-        f16x8 vf[3], vr[3];
+        f16x8 vf[PD + 1], vr[PD + 1];
 #pragma unroll
-        for (uint32_t m = 0; m < 2; m++) {
+        for (uint32_t m = 0; m < PD; m++) {
             vf[m] = fr(KF + m * 1024);
             if constexpr (NS == 2) vr[m] = fr(KF + VF + m * 1024);
         }
 #pragma unroll
         for (uint32_t m = 0; m < 2 * NB; m++) {   // block m / 2, keys 16 (m % 2) ..
             const uint32_t b = m / 2, s = m & 1u;
-            const f16x8 v = vf[m % 3], r = vr[m % 3];
-            if (m + 2 < 2 * NB) {
-                vf[(m + 2) % 3] = fr(KF + (m + 2) * 1024);
-                if constexpr (NS == 2) vr[(m + 2) % 3] = fr(KF + VF + (m + 2) * 1024);
+            const f16x8 v = vf[m % (PD + 1)], r = vr[m % (PD + 1)];
+            if (m + PD < 2 * NB) {
+                vf[(m + PD) % (PD + 1)] = fr(KF + (m + PD) * 1024);
+                if constexpr (NS == 2) vr[(m + PD) % (PD + 1)] = fr(KF + VF + (m + PD) * 1024);
             }
             O[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, P[0][s], O[b], 0, 0, 0);
             if constexpr (NP == 2) O[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, P[NP - 1][s], O[b], 0, 0, 0);
@@ -1660,22 +1664,18 @@ __global__ __launch_bounds__(64 * NW, T == SINTER_F32 ? 1 : 2) void kv4_tile_ker
         issue(0, in);
         dma_wait();
         __syncthreads();
-        unpack(0, in);
+#pragma unroll
+        for (uint32_t p = 0; p < PIECES; p++) unpack(0, in, p, lane);
         uint32_t holes = in.holes;
         if (n_tile > 1) issue(1, in);
         for (int j = 0; j < n_tile; j++) {
             dma_wait();        // tile j + 1's loads, issued an iteration ago
             __syncthreads();   // they are in from every wave; tile j is unpacked; tile j - 1 is done with
-            // The two waves of a SIMD take turns: one unpacks (VALU) while the
-            // other's scores run on the matrix core, and so on through a tile
+            // (behind the last tile its own loads are unpacked again, for nobody)
             const uint32_t h = in.holes;
-            auto fetch = [&] {
-                if (j + 1 < n_tile) unpack(j + 1, in);
-                if (j + 2 < n_tile) issue(j + 2, in);
-            };
-            if (NW == 4 || w < 4) fetch();
-            compute(j, holes);
-            if (NW == 8 && w >= 4) fetch();
+            if (!MIX && w < 4) fetch(j, in);
+            compute(j, holes, in);
+            if (!MIX && w >= 4) fetch(j, in);
             holes = h;
         }
     }
