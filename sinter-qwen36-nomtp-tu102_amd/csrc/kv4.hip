@@ -1091,11 +1091,15 @@ __global__ __launch_bounds__(64 * NW) void kv4_merge_kernel(Attn a, uint32_t row
     __shared__ __attribute__((aligned(16))) float comb[NW][256];
     const uint32_t r = blockIdx.x % rows, sg = blockIdx.x / rows, g = sg % a.b.nkv, lane = threadIdx.x & 63u, HD = a.b.hd;
     const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // Most of a mixed batch's workgroups have no such row: they leave at once
+    const uint32_t seq = sg / a.b.nkv;
+    const int rows_of = (a.b.tok_start[seq + 1] - a.b.tok_start[seq]) * (int)a.gqa;
+    if ((int)r >= rows_of || rows_of > (int)a.split_rows || a.b.kv_len[seq] <= (int)(WHOLE * TILE)) return;
     // (one wave looks the parts up: sixteen at it would take turns)
     __shared__ uint32_t place[4];   // parts, the first one's slot, whether that is the slot's second record, first token
     if (w == 0) {
         Deal d;
-        const Work wk = deal(a, sg / a.b.nkv, true, d);
+        const Work wk = deal(a, seq, true, d);
         uint32_t n = 0, i0 = 0, second = 0;
         if (wk.seq >= 0 && r < (uint32_t)wk.n_new * a.gqa) {
             const uint32_t tiles = seg_tiles(a, wk.len), units = seg_units(tiles, d.tiles), begin = wk.first + r / 16 * units;
@@ -1252,7 +1256,7 @@ __device__ __forceinline__ uint32_t chunk_rows(uint32_t seen, uint32_t n_split) 
 // block's sums of the rows that do.
 //
 // Bound by a wave's instructions and waits beside the matrix core, which is busy
-// a third of the time: 500 tokens of 24 heads of 256 over 4 behind 32,000 rows,
+// a quarter (bf16) to a third (F32) of the time: 500 tokens of 24 heads of 256 over 4 behind 32,000 rows,
 // F32: 1344 us, 295 TF/s and with each product in three parts 885 TF/s of f16 (a
 // large f16 product: 1166); bf16: 530 us, 750 TF/s.  Two prompts of 2000 tokens,
 // bf16: 163 us, 640 TF/s.
