@@ -483,10 +483,10 @@ __device__ __forceinline__ uint32_t row_cap(const Attn &a) {
     return (uint32_t)min((uint64_t)a.max_kv, (uint64_t)a.b.max_pages << a.page_shift);
 }
 
-// sequence base + lane: its rows, first token and tokens (0: none, or none of
-// them within the arrays).  report: raise the error of lengths over the bounds
-__device__ __forceinline__ void load_seq(const Attn &a, uint32_t base, bool report, int &len, int &t0, int &n) {
-    const uint32_t s = base + (threadIdx.x & 63u), i = min(s, a.b.n_seq - 1u);
+// sequence s: its rows, first token and tokens (0: none, or none of them within
+// the arrays).  report: raise the error of lengths over the bounds
+__device__ __forceinline__ void load_one(const Attn &a, uint32_t s, bool report, int &len, int &t0, int &n) {
+    const uint32_t i = min(s, a.b.n_seq - 1u);
     t0 = a.b.tok_start[i];
     n = a.b.tok_start[i + 1] - t0;
     len = a.b.kv_len[i];
@@ -497,6 +497,11 @@ __device__ __forceinline__ void load_seq(const Attn &a, uint32_t base, bool repo
     if (t0 < 0 || n <= 0 || (uint32_t)t0 >= a.b.n_tok) n = 0;
     else n = min(n, (int)(a.b.n_tok - (uint32_t)t0));
     len = max(0, len);
+}
+
+// sequence base + lane
+__device__ __forceinline__ void load_seq(const Attn &a, uint32_t base, bool report, int &len, int &t0, int &n) {
+    load_one(a, base + (threadIdx.x & 63u), report, len, t0, n);
 }
 
 // inclusive sum over the lanes (every lane active)
@@ -616,24 +621,39 @@ __device__ __forceinline__ Work deal(const Attn &a, uint32_t id, bool by_seq, De
         pick(w, 0, by_seq ? id : id * d.share, by_seq, len, t0, n, c, sum - c);
         return w;
     }
-    uint32_t total = 0, segs = 0;
-#pragma unroll 4
-    for (uint32_t base = 0; base < a.b.n_seq; base += 64) {   // (four loads in flight)
-        load_seq(a, base, false, len, t0, n);
+    // More: a lane counts `per` sequences in a row (eight loads in flight), and
+    // the search goes through one lane's (2048 replies behind 300 rows, 32 heads of
+    // 128 over 8, bf16: 272 us, sixty-four at a time, one load after the other, 280)
+    const uint32_t lane = threadIdx.x & 63u, per = (a.b.n_seq + 63u) / 64u;
+    uint32_t mine = 0, segs = 0;
+#pragma unroll 8
+    for (uint32_t i = 0; i < per; i++) {
+        load_one(a, lane * per + i, false, len, t0, n);
         const uint32_t mts = row_tiles(a, n);
-        total += wave_sum_u32(mts * seg_tiles(a, len));
-        segs += wave_sum_u32(mts);
+        mine += mts * seg_tiles(a, len);
+        segs += mts;
     }
-    d = deal_of(a, total, segs);
+    d = deal_of(a, wave_sum_u32(mine), wave_sum_u32(segs));
     if (d.tiles > 1u) {
-        d.total = 0;
-#pragma unroll 4
-        for (uint32_t base = 0; base < a.b.n_seq; base += 64) {
-            load_seq(a, base, false, len, t0, n);
-            d.total += wave_sum_u32(row_tiles(a, n) * seg_units(seg_tiles(a, len), d.tiles));
+        mine = 0;
+#pragma unroll 8
+        for (uint32_t i = 0; i < per; i++) {
+            load_one(a, lane * per + i, false, len, t0, n);
+            mine += row_tiles(a, n) * seg_units(seg_tiles(a, len), d.tiles);
         }
     }
-    return find_units(a, d, by_seq ? id : id * d.share, by_seq);
+    const uint32_t sum = wave_scan_u32(mine), at = by_seq ? id : id * d.share;
+    d.total = (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+    const uint64_t m = __builtin_amdgcn_ballot_w64(by_seq ? id >= lane * per && id < (lane + 1u) * per : at >= sum - mine && at < sum);
+    Work from;
+    from.base = a.b.n_seq;   // (none)
+    from.before = 0;
+    if (m != 0) {
+        const int l = __builtin_ctzll(m);
+        from.base = (uint32_t)l * per;
+        from.before = (uint32_t)__builtin_amdgcn_readlane((int)(sum - mine), l);
+    }
+    return find_units(a, d, at, by_seq, &from);
 }
 
 // the gated, normalised output of four elements
