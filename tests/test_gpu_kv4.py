@@ -353,6 +353,31 @@ def test_attention_many_sequences(sn, torch_gpu, n_seq):
     check_attn(b, 2, BF16, q, got, g, 64 ** -0.5)
 
 
+@pytest.mark.parametrize("t,nkv,hd,n_seq", [(F32, 16, 256, 40), (BF16, 8, 256, 80), (F16, 16, 64, 70)])
+def test_attention_more_sequences_than_slots(sn, torch_gpu, t, nkv, hd, n_seq):
+    """Long sequences that share the slots of a call, each divided where a
+    slot's share ends; all read one sequence's pages."""
+    torch = torch_gpu
+    rng = np.random.default_rng(hd + n_seq)
+    kv = rng.integers(500, 1200, n_seq)
+    kv[0], kv[5], kv[7] = 1200, 1, 40
+    new = np.ones(n_seq, int)
+    new[3], new[9] = 2, 0
+    b = Batch(sn, torch, list(new), list(kv), 64, nkv, hd, seed=n_seq)
+    b.pages[:] = b.pages[0]
+    b.kv_len = b.kv_len[:1]
+    b.fill_rows(7)
+    b.kv_len = kv.astype(np.int32)
+    b.up()
+    q = rng.standard_normal((b.n_tok, nkv, hd)).astype(np.float32)
+    (_, qv), (_, ov) = strided(torch, q, t), strided(torch, np.full(q.shape, 3.0, np.float32), t)
+    a, ws = attn_args(sn, torch, b, nkv, t, qv, ov)
+    print(f"{n_seq} sequences over {nkv} heads of {hd}", flush=True)
+    ok(sn, sn.lib().sinter_kv4_attn(C.byref(b.rec()), C.byref(a), stream(torch)), torch)
+    check_attn(b, nkv, t, qv.double().cpu().numpy(), ov.float().cpu().numpy(), None, hd ** -0.5,
+               only={0, 3, 4, 5, 7, *range(9, b.n_tok, 9)})
+
+
 @pytest.mark.parametrize("t", [F32, BF16])
 def test_attention_many_sequences_of_many_rows(sn, torch_gpu, t):
     """More than 64 sequences, prompts among them, empty ones between."""
@@ -797,6 +822,31 @@ def test_two_streams_at_once(sn, torch_gpu):
     torch.cuda.synchronize()
     assert torch.equal(outs[0], outs[1]) and sn.op_error()[0] == 0
     check_attn(b, 8, F32, q.double().cpu().numpy(), outs[0].cpu().numpy(), None, 128 ** -0.5)
+
+
+def test_two_streams_at_once_of_many_rows(sn, torch_gpu):
+    """Prompts on one stream, replies and another step's append on the other."""
+    torch = torch_gpu
+    many, few = Batch(sn, torch, [150, 90], [700, 300], 64, 2, 64, seed=2), Batch(sn, torch, [1, 2], [1500, 40], 64, 2, 64, seed=3)
+    qs, outs, runs = [], [], []
+    for b in (many, few):
+        b.fill_rows(3)
+        q = torch.randn(b.n_tok, 8, 64, device="cuda", dtype=torch.float16)
+        out = torch.zeros_like(q)
+        qs.append(q), outs.append(out)
+        runs.append((torch.cuda.Stream(), b.rec(), *attn_args(sn, torch, b, 8, F16, q, out)))
+    other = Batch(sn, torch, [40, 40], [40, 64], 16, 2, 64, seed=4)
+    x = torch.randn(80, 2, 64, device="cuda")
+    torch.cuda.synchronize()
+    L = sn.lib()
+    for _ in range(10):
+        for s, r, a, ws in runs:
+            sn.check(L.sinter_kv4_attn(C.byref(r), C.byref(a), C.c_void_p(s.cuda_stream)))
+        sn.check(L.sinter_kv4_append(C.byref(other.rec()), C.byref(heads(sn, x)), C.byref(heads(sn, x)), F32, C.c_void_p(runs[1][0].cuda_stream)))
+    torch.cuda.synchronize()
+    assert sn.op_error()[0] == 0
+    for b, q, out, n in zip((many, few), qs, outs, (11, 1)):
+        check_attn(b, 8, F16, q.double().cpu().numpy(), out.float().cpu().numpy(), None, 0.125, only=set(range(0, b.n_tok, n)))
 
 
 def test_same_bits_every_time(sn, torch_gpu):
